@@ -330,7 +330,7 @@ def _plain_plan(s):
     grow = new.clamp(min=0)
     end = torch.cumsum(grow, 0)
     used = (cached + bs - 1) // bs
-    fits = (new >= 0) & (cached >= 0) & (cached + grow <= W * bs) & (end <= cap)
+    fits = (new >= 0) & (cached >= 0) & (cached + grow <= W * bs) & ((new == 0) | (end <= cap))
     need = torch.where(fits, (cached + grow + bs - 1) // bs - used, 0)
     cum = torch.cumsum(need, 0)
     ok = fits & ((need == 0) | (cum <= count))
