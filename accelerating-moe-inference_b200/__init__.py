@@ -41,6 +41,11 @@ GEMM_AUTO = 0
 GEMM_SINGLE_CTA = 1
 GEMM_CTA_PAIR = 2
 
+# MoeDtype: element type of the 4-bit operators' activations.
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+DTYPE_F16 = 2
+
 # Every symbol include/moe_b200.h declares.
 EXPORTED_SYMBOLS = (
     "moe_abi_version", "moe_last_error", "moe_config_init", "moe_create", "moe_create_from_device",
@@ -56,6 +61,11 @@ EXPORTED_SYMBOLS = (
     "moe_decoder_create_from_device", "moe_decoder_destroy", "moe_decoder_device_bytes",
     "moe_decoder_prefill", "moe_decoder_decode_step", "moe_decoder_generate",
     "moe_decoder_last_timing", "moe_decoder_set_fused_step", "moe_decoder_fused_step_active",
+    "moe_kv4_config_init", "moe_kv4_create", "moe_kv4_destroy", "moe_kv4_cache_bytes",
+    "moe_kv4_device_bytes", "moe_kv4_plan_device", "moe_kv4_append_device",
+    "moe_kv4_attention_device",
+    "moe_w4_config_init", "moe_w4_create", "moe_w4_create_from_device", "moe_w4_destroy",
+    "moe_w4_device_bytes", "moe_w4_matvec_device", "moe_w4_experts_device",
 )
 PROFILE_STAGES = ("router", "dispatch_scan", "dispatch_permute", "gateup_gemm", "down_gemm",
                   "ep_exchange_in", "ep_exchange_out", "ep_combine")
@@ -97,6 +107,20 @@ class MoeDecoderConfig(ctypes.Structure):
                 ("precision", ctypes.c_int32), ("max_batch", ctypes.c_int32),
                 ("max_seq", ctypes.c_int32), ("device", ctypes.c_int32),
                 ("reserved", ctypes.c_int32 * 4)]
+
+
+class MoeKv4Config(ctypes.Structure):
+    _fields_ = [("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("block_tokens", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("max_requests", ctypes.c_int32),
+                ("device", ctypes.c_int32), ("reserved", ctypes.c_int32 * 5)]
+
+
+class MoeW4Config(ctypes.Structure):
+    _fields_ = [("num_matrices", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("cols", ctypes.c_int32), ("group", ctypes.c_int32), ("gated", ctypes.c_int32),
+                ("device", ctypes.c_int32), ("max_rows", ctypes.c_int32),
+                ("reserved", ctypes.c_int32 * 5)]
 
 
 _f32pp = ctypes.POINTER(_f32p)
@@ -180,6 +204,32 @@ def load_library(path: Optional[Path] = None) -> ctypes.CDLL:
     L.moe_decoder_last_timing.argtypes = [vp, _f32p, _f32p]
     L.moe_decoder_set_fused_step.argtypes = [vp, ctypes.c_int32]
     L.moe_decoder_fused_step_active.argtypes = [vp]
+    i32, i64, f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+    L.moe_kv4_config_init.argtypes = [ctypes.POINTER(MoeKv4Config)]
+    L.moe_kv4_config_init.restype = None
+    L.moe_kv4_create.argtypes = [ctypes.POINTER(MoeKv4Config), ctypes.POINTER(vp)]
+    L.moe_kv4_destroy.argtypes = [vp]
+    L.moe_kv4_destroy.restype = None
+    L.moe_kv4_cache_bytes.argtypes = [vp]
+    L.moe_kv4_cache_bytes.restype = ctypes.c_size_t
+    L.moe_kv4_device_bytes.argtypes = [vp]
+    L.moe_kv4_device_bytes.restype = ctypes.c_size_t
+    L.moe_kv4_plan_device.argtypes = [vp, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp]
+    L.moe_kv4_append_device.argtypes = [vp, vp, vp, vp, i32, i32, i64, i64, i64, i64, vp, vp, vp,
+                                        vp]
+    L.moe_kv4_attention_device.argtypes = [vp, vp, vp, i32, i32, i32, i64, i64, vp, vp, vp, i32,
+                                           f32, i32, vp, vp, vp]
+    wcp = ctypes.POINTER(MoeW4Config)
+    L.moe_w4_config_init.argtypes = [wcp]
+    L.moe_w4_config_init.restype = None
+    L.moe_w4_create.argtypes = [wcp, vp, vp, vp, ctypes.POINTER(vp)]
+    L.moe_w4_create_from_device.argtypes = L.moe_w4_create.argtypes
+    L.moe_w4_destroy.argtypes = [vp]
+    L.moe_w4_destroy.restype = None
+    L.moe_w4_device_bytes.argtypes = [vp]
+    L.moe_w4_device_bytes.restype = ctypes.c_size_t
+    L.moe_w4_matvec_device.argtypes = [vp, vp, i32, i32, i64, i32, vp, vp, vp]
+    L.moe_w4_experts_device.argtypes = [vp, vp, vp, i32, i32, i32, vp, vp, vp, vp]
     if path is None:
         _lib = L
     return L
@@ -798,3 +848,208 @@ class MoeDecoder:
 
     def __exit__(self, *a):
         self.close()
+
+
+# ---------------------------------------------------------------------------
+# A decode step in 4 bits: moe_kv4_* and moe_w4_* in include/moe_b200.h.
+# Pointers are integer device addresses, dtype one of DTYPE_F32 / BF16 / F16.
+
+class Kv4Cache:
+    """Geometry and workspace of a paged 4-bit key/value cache (moe_kv4_*).
+    The cache buffers (cache_bytes() each, one per layer) are the caller's."""
+
+    def __init__(self, *, num_kv_heads: int, head_dim: int, block_tokens: int, num_blocks: int,
+                 table_width: int, max_requests: int, device: int = 0):
+        L = load_library()
+        cfg = MoeKv4Config()
+        L.moe_kv4_config_init(ctypes.byref(cfg))
+        cfg.num_kv_heads, cfg.head_dim, cfg.block_tokens = num_kv_heads, head_dim, block_tokens
+        cfg.num_blocks, cfg.table_width, cfg.max_requests = num_blocks, table_width, max_requests
+        cfg.device = device
+        self._h = None
+        h = ctypes.c_void_p()
+        _check(L.moe_kv4_create(ctypes.byref(cfg), ctypes.byref(h)))
+        self._h = h
+        self.cfg = cfg
+        self._lib = L
+
+    def cache_bytes(self) -> int:
+        """Bytes of one cache buffer."""
+        return self._lib.moe_kv4_cache_bytes(self._h)
+
+    def device_bytes(self) -> int:
+        """Bytes of the attention's workspace."""
+        return self._lib.moe_kv4_device_bytes(self._h)
+
+    def plan(self, cached_len_ptr: int, new_len_ptr: int, num_requests: int, free_ring_ptr: int,
+             ring_state_ptr: int, block_table_ptr: int, kv_len_ptr: int, q_offset_ptr: int,
+             position_ptr: int, slot_ptr: int, tokens_cap: int, ring_state_out_ptr: int,
+             stream: int = 0):
+        """Block tables and slot map of one step (moe_kv4_plan_device)."""
+        rc = self._lib.moe_kv4_plan_device(
+            self._h, cached_len_ptr, new_len_ptr, num_requests, free_ring_ptr, ring_state_ptr,
+            block_table_ptr, kv_len_ptr, q_offset_ptr, position_ptr, slot_ptr, tokens_cap,
+            ring_state_out_ptr, stream)
+        if rc:
+            _check(rc)
+
+    def append(self, cache_ptr: int, k_ptr: int, v_ptr: int, dtype: int, tokens: int,
+               slot_ptr: int, stream: int = 0, *, k_strides=None, v_strides=None,
+               k_out_ptr: int = 0, v_out_ptr: int = 0):
+        """Quantise keys and values into their slots (moe_kv4_append_device).
+        k_strides / v_strides: (token, head) strides in elements, contiguous
+        [tokens][num_kv_heads][head_dim] by default."""
+        if k_strides is None or v_strides is None:
+            dense = (self.cfg.num_kv_heads * self.cfg.head_dim, self.cfg.head_dim)
+            k_strides, v_strides = k_strides or dense, v_strides or dense
+        rc = self._lib.moe_kv4_append_device(
+            self._h, cache_ptr, k_ptr, v_ptr, dtype, tokens, k_strides[0], k_strides[1],
+            v_strides[0], v_strides[1], slot_ptr, k_out_ptr, v_out_ptr, stream)
+        if rc:
+            _check(rc)
+
+    def attention(self, cache_ptr: int, q_ptr: int, out_ptr: int, dtype: int, tokens: int,
+                  num_heads: int, block_table_ptr: int, kv_len_ptr: int, q_offset_ptr: int,
+                  num_requests: int, stream: int = 0, *, scale: Optional[float] = None,
+                  window: int = 0, q_strides=None, lse_ptr: int = 0):
+        """Attention of the packed query tokens over the cache
+        (moe_kv4_attention_device); scale 1 / sqrt(head_dim) by default."""
+        hd = self.cfg.head_dim
+        if q_strides is None:
+            q_strides = (num_heads * hd, hd)
+        rc = self._lib.moe_kv4_attention_device(
+            self._h, cache_ptr, q_ptr, dtype, tokens, num_heads, q_strides[0], q_strides[1],
+            block_table_ptr, kv_len_ptr, q_offset_ptr, num_requests,
+            hd ** -0.5 if scale is None else scale, window, out_ptr, lse_ptr, stream)
+        if rc:
+            _check(rc)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._lib.moe_kv4_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+
+def quantize_w4(w: np.ndarray, group: int = 128, zeros: bool = True):
+    """fp32 weights [..., rows][cols] -> (codes [..., rows][cols / 2] uint8,
+    scales [..., rows][ceil(cols / group)] float16, zeros of that shape uint8 or
+    None): w ~ scale * (code - zero), zero 8 without zeros."""
+    w = np.asarray(w, np.float32)
+    K = w.shape[-1]
+    if K % 32 or group not in (32, 64, 128):
+        raise ValueError("cols must be a multiple of 32 and group 32, 64 or 128")
+    G = -(-K // group)
+    at = np.arange(K) // group
+    pad = np.concatenate([w, np.repeat(w[..., -1:], G * group - K, -1)], -1)
+    pad = pad.reshape(*w.shape[:-1], G, group)
+    if zeros:
+        lo, hi = np.minimum(pad.min(-1), 0), np.maximum(pad.max(-1), 0)
+        s = ((hi - lo) / 15).astype(np.float16)
+        safe = np.where(s > 0, s.astype(np.float32), 1)
+        z = np.clip(np.rint(-lo / safe), 0, 15).astype(np.uint8)
+    else:
+        s = (np.abs(pad).max(-1) / 7.5).astype(np.float16)
+        safe = np.where(s > 0, s.astype(np.float32), 1)
+        z = np.full(s.shape, 8, np.uint8)
+    c = np.clip(np.rint(w / safe[..., at]) + z[..., at], 0, 15).astype(np.uint8)
+    return c[..., 0::2] | (c[..., 1::2] << 4), s, z if zeros else None
+
+
+class W4Matrix:
+    """One or several equally shaped matrices of 4-bit weights (moe_w4_*)."""
+
+    def __init__(self, codes: np.ndarray, scales: np.ndarray, zeros: Optional[np.ndarray] = None,
+                 *, group: int = 128, gated: bool = False, device: int = 0, max_rows: int = 16):
+        """Host arrays as quantize_w4 gives them, [matrices][rows][...] (or
+        [rows][...] for one matrix)."""
+        codes = np.ascontiguousarray(codes, np.uint8)
+        codes = codes[None] if codes.ndim == 2 else codes
+        E, N, K = codes.shape[0], codes.shape[1], codes.shape[2] * 2
+        shape = (E, N, -(-K // group))
+        scales = np.ascontiguousarray(scales, np.float16).reshape(-1)
+        zeros = None if zeros is None else np.ascontiguousarray(zeros, np.uint8).reshape(-1)
+        for a in (scales, zeros):
+            if a is not None and a.size != int(np.prod(shape)):
+                raise ValueError(f"scales and zeros must have shape {shape}")
+        self._create(load_library().moe_w4_create, codes.ctypes.data, scales.ctypes.data,
+                     None if zeros is None else zeros.ctypes.data, E, N, K, group, gated, device,
+                     max_rows)
+
+    @classmethod
+    def from_device_pointers(cls, codes_ptr: int, scales_ptr: int, zeros_ptr: int = 0, *,
+                             matrices: int, rows: int, cols: int, group: int = 128,
+                             gated: bool = False, device: int = 0,
+                             max_rows: int = 16) -> "W4Matrix":
+        """The same from device arrays (moe_w4_create_from_device)."""
+        self = cls.__new__(cls)
+        self._create(load_library().moe_w4_create_from_device, codes_ptr, scales_ptr,
+                     zeros_ptr or None, matrices, rows, cols, group, gated, device, max_rows)
+        return self
+
+    def _create(self, fn, codes, scales, zeros, E, N, K, group, gated, device, max_rows):
+        L = load_library()
+        cfg = MoeW4Config()
+        L.moe_w4_config_init(ctypes.byref(cfg))
+        cfg.num_matrices, cfg.rows, cfg.cols, cfg.group = E, N, K, group
+        cfg.gated, cfg.device, cfg.max_rows = int(gated), device, max_rows
+        self._h = None
+        h = ctypes.c_void_p()
+        _check(fn(ctypes.byref(cfg), codes, scales, zeros, ctypes.byref(h)))
+        self._h = h
+        self.cfg = cfg
+        self._lib = L
+
+    @property
+    def outputs(self) -> int:
+        return self.cfg.rows // 2 if self.cfg.gated else self.cfg.rows
+
+    def device_bytes(self) -> int:
+        return self._lib.moe_w4_device_bytes(self._h)
+
+    def matvec(self, x_ptr: int, y_ptr: int, num_rows: int, dtype: int, stream: int = 0, *,
+               matrix_ptr: int = 0, x_row_stride: Optional[int] = None, x_share: int = 1):
+        """y[i] = matrix[i] x[i // x_share] (moe_w4_matvec_device)."""
+        rc = self._lib.moe_w4_matvec_device(
+            self._h, x_ptr, dtype, num_rows,
+            self.cfg.cols if x_row_stride is None else x_row_stride, x_share, matrix_ptr, y_ptr,
+            stream)
+        if rc:
+            _check(rc)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._lib.moe_w4_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+
+def w4_experts(gate_up: W4Matrix, down: W4Matrix, x_ptr: int, idx_ptr: int, weights_ptr: int,
+               y_ptr: int, num_tokens: int, top_k: int, dtype: int, stream: int = 0) -> None:
+    """The routed experts on 4-bit weights (moe_w4_experts_device)."""
+    rc = gate_up._lib.moe_w4_experts_device(gate_up._h, down._h, x_ptr, dtype, num_tokens, top_k,
+                                            idx_ptr, weights_ptr, y_ptr, stream)
+    if rc:
+        _check(rc)

@@ -487,6 +487,191 @@ int moe_decoder_set_fused_step(MoeDecoder* m, int32_t enable);
 /* 1 if batch-1 decode steps run the fused step, else 0 (or a null m). */
 int moe_decoder_fused_step_active(const MoeDecoder* m);
 
+/* ---------------------------------------------------------------------
+ * A decode step in 4 bits (no counterpart in the reference, whose weights and
+ * activations are fp32 and which keeps no cache): a paged key/value cache of
+ * 4-bit codes with the block tables that address it, attention over it, and
+ * matrix-vector products and routed experts on 4-bit weights.
+ *
+ * All entry points below take device pointers, enqueue on `stream` and do not
+ * synchronise; they check what the host can see (sizes, types, alignment,
+ * null pointers) and return MOE_ERR_INVALID / MOE_ERR_UNSUPPORTED before any
+ * launch.  Device-side indexes (block ids, slots, expert ids, lengths) are
+ * bounds-checked by the kernels as stated at each call. */
+
+/* Element type of activations, queries, keys and values. */
+typedef enum MoeDtype {
+    MOE_DTYPE_F32 = 0,
+    MOE_DTYPE_BF16 = 1,
+    MOE_DTYPE_F16 = 2
+} MoeDtype;
+
+/* ---- The paged 4-bit key/value cache.
+ *
+ * A group of 64 consecutive dims of one token's key (or value) of one head is
+ * stored as 64 4-bit codes c with a float16 scale s and minimum m; a code
+ * stands for s * c + m.  A page holds block_tokens tokens of every head; the
+ * cache buffer (the caller's, one per layer, 16-byte aligned,
+ * moe_kv4_cache_bytes) is [num_blocks][num_kv_heads][block_tokens / 16]
+ * granules of 16 tokens of one head, each 16 * D + 128 * (D / 64) bytes
+ * (D = head_dim, G = D / 64):
+ *   K codes   [16 tokens][4 j][G g][2 h][4 bytes]: byte b of (j, g, h) holds
+ *             dims 64 g + 16 j + 8 h + 2 b (low nibble) and + 1
+ *   V codes   [G p][8 n][4 j][4 / G v][G g][4 bytes]: of token
+ *             8 (u / 2) + 2 j + u % 2, u = p * (4 / G) + v, byte b of g holds
+ *             dims 64 g + 8 n + 2 b (low nibble) and + 1
+ *   K params  [16 tokens][G] (scale, minimum) float16 pairs
+ *   V params  the same
+ * Bytes of tokens that were never appended may hold anything. */
+typedef struct MoeKv4Config {
+    int32_t num_kv_heads;  /* 1..256 */
+    int32_t head_dim;      /* 64 or 128 */
+    int32_t block_tokens;  /* tokens per page: a multiple of 16, at most 1024 */
+    int32_t num_blocks;    /* pages of the pool */
+    int32_t table_width;   /* block-table entries per request */
+    int32_t max_requests;  /* requests per call, 1..8192 */
+    int32_t device;
+    int32_t reserved[5];
+} MoeKv4Config;
+
+typedef struct MoeKv4 MoeKv4;
+
+/* Defaults: 16 heads of 128 (the toy decoder), pages of 16 tokens, 640
+ * positions and 16 requests, a pool that holds them all, device 0. */
+void moe_kv4_config_init(MoeKv4Config* cfg);
+/* The handle holds the geometry and the attention's workspace, no cache: one
+ * handle serves every layer of a model.  One stream at a time. */
+int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out);
+void moe_kv4_destroy(MoeKv4* h);
+/* Bytes of one cache buffer, and of the handle's workspace (0 for null). */
+size_t moe_kv4_cache_bytes(const MoeKv4* h);
+size_t moe_kv4_device_bytes(const MoeKv4* h);
+
+/* Block tables and slot maps of one step, from the requests' lengths.
+ *   cached_len [R]   tokens request r has in the cache
+ *   new_len [R]      tokens this step adds to it (0: none; negative: the
+ *                    request ends and its pages go back to the pool)
+ *   free_ring [num_blocks], ring_state [2] = {head, count}: the free pages are
+ *                    free_ring[(head + i) % num_blocks], i < count
+ *   block_table [R][table_width]  in: the pages of the cached tokens; the
+ *                    step's new pages are written behind them
+ * A request that needs need = ceil((cached + new) / block_tokens) -
+ * ceil(cached / block_tokens) pages takes them from the ring's front, in
+ * request order.  It is rejected if a length is out of range (cached < 0, or
+ * cached + new beyond table_width pages), if its tokens would lie at or past
+ * tokens_cap in the step's packed tokens, or if it needs pages and the needs
+ * up to and including its own exceed count.  Freed pages are appended behind
+ * the ring's last one, in request order, and can be taken from the next step
+ * on; the table rows of ended requests are left as they are.
+ * Outputs:
+ *   kv_len [R]       cached + new; 0 for rejected and ended requests
+ *   q_offset [R+1]   first packed token of each request (rejected ones keep
+ *                    their tokens' places), clipped to tokens_cap
+ *   position [tokens_cap]  position of each packed token in its request; -1
+ *                    behind the last one
+ *   slot [tokens_cap]  page * block_tokens + offset in the page; -1 for tokens
+ *                    of rejected requests, behind the last token, and where
+ *                    the table holds a page outside the pool
+ *   ring_state_out [2]  the state after the step (not ring_state itself)
+ * Inputs are not changed other than table and ring as stated, so a step may
+ * be planned again.  A ring_state outside 0 <= head < num_blocks,
+ * 0 <= count <= num_blocks counts as an empty ring at 0. */
+int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new_len,
+                        int32_t num_requests, int32_t* free_ring, const int32_t* ring_state,
+                        int32_t* block_table, int32_t* kv_len, int32_t* q_offset,
+                        int32_t* position, int64_t* slot, int32_t tokens_cap,
+                        int32_t* ring_state_out, void* stream);
+
+/* Quantises the keys and values of `tokens` tokens into the cache at their
+ * slots.  k, v: [tokens][num_kv_heads][head_dim] of `dtype`, strides in
+ * elements, the last dim contiguous.  Per group of 64 dims, each step rounded
+ * to fp32: x clamped to +-65504, s = f16((max - min) * (1/15)),
+ * m = f16(min), c = rint((x - m) / s) within 0..15 (0 where s is 0).  A group
+ * that holds a NaN gets s = m = NaN and codes 0.  Tokens with a slot outside
+ * [0, num_blocks * block_tokens) are not stored; two tokens of a call must not
+ * share a slot.  k_out / v_out (either may be null): the values the codes
+ * stand for, [tokens][num_kv_heads][head_dim] contiguous in `dtype`, for every
+ * token. */
+int moe_kv4_append_device(MoeKv4* h, void* cache, const void* k, const void* v, int32_t dtype,
+                          int32_t tokens, int64_t k_token_stride, int64_t k_head_stride,
+                          int64_t v_token_stride, int64_t v_head_stride, const int64_t* slot,
+                          void* k_out, void* v_out, void* stream);
+
+/* out[t] = attention of the packed query tokens over the cache.
+ * Request r's queries are tokens q_offset[r] .. q_offset[r+1] - 1 (within
+ * [0, tokens)), the last of them at position kv_len[r] - 1; a query at
+ * position p sees the keys at positions max(0, p - window + 1) .. p (window 0:
+ * all up to p).  Query head i reads key/value head i / (num_heads /
+ * num_kv_heads); num_heads is a multiple of num_kv_heads, at most 64 times it.
+ * q: [tokens][num_heads][head_dim], strides in elements; out: contiguous, of
+ * the same type; lse [tokens][num_heads] fp32 (may be null): log of the sum of
+ * exp of the scaled scores.  A query that sees no key gets out 0 and lse -inf;
+ * tokens behind q_offset[num_requests] are not written.  kv_len beyond the
+ * table's width is cut to it; keys on a page outside the pool are not seen.
+ * Scores, softmax and sums are in fp32; q and the probabilities enter the
+ * products as float16 with 11 significant bits for 16-bit types and 22 for
+ * fp32. */
+int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_t dtype,
+                             int32_t tokens, int32_t num_heads, int64_t q_token_stride,
+                             int64_t q_head_stride, const int32_t* block_table,
+                             const int32_t* kv_len, const int32_t* q_offset,
+                             int32_t num_requests, float scale, int32_t window, void* out,
+                             float* lse, void* stream);
+
+/* ---- Matrix-vector products with 4-bit weights.
+ *
+ * num_matrices matrices of [rows][cols]; weight (n, k) of a matrix is
+ * scales[n][k / group] * (code - zero), zero = zeros[n][k / group], 8 without
+ * zeros.  gated: the rows are two halves, gate rows then up rows, and a
+ * product gives silu(gate) * up, rows / 2 values. */
+typedef struct MoeW4Config {
+    int32_t num_matrices;  /* 1..256 */
+    int32_t rows;          /* outputs; even if gated */
+    int32_t cols;          /* inputs: a multiple of 32, at most 65536 */
+    int32_t group;         /* 32, 64 or 128 */
+    int32_t gated;
+    int32_t device;
+    int32_t max_rows;      /* workspace is pre-sized for this many product rows; grows on demand */
+    int32_t reserved[5];
+} MoeW4Config;
+
+typedef struct MoeW4 MoeW4;
+
+/* One matrix of 4096 x 4096, group 128, device 0, 16 product rows. */
+void moe_w4_config_init(MoeW4Config* cfg);
+/* From codes [num_matrices][rows][cols / 2] (two codes per byte, the even
+ * column in the low nibble), scales [num_matrices][rows][ceil(cols / group)]
+ * float16 and zeros (uint8, 0..15, the same shape; may be null), on the host
+ * or on cfg->device.  Copied; the caller keeps ownership. */
+int moe_w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales,
+                  const uint8_t* zeros, MoeW4** out);
+int moe_w4_create_from_device(const MoeW4Config* cfg, const uint8_t* codes, const void* scales,
+                              const uint8_t* zeros, MoeW4** out);
+void moe_w4_destroy(MoeW4* h);
+size_t moe_w4_device_bytes(const MoeW4* h);
+
+/* y[i] = matrix[i] * x[i / x_share], i < num_rows (0..512): x
+ * [ceil(num_rows / x_share)][cols] with a row stride in elements, y
+ * [num_rows][outputs] contiguous, both of `dtype`.  matrix [num_rows] (device,
+ * may be null: matrix 0): the matrix of each product; a row whose entry is
+ * outside [0, num_matrices) gets zeros.  Sums are in fp32; x enters the
+ * products exactly. */
+int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_rows,
+                         int64_t x_row_stride, int32_t x_share, const int32_t* matrix, void* y,
+                         void* stream);
+
+/* The routed experts on 4-bit weights: y[t] = sum over s of weights[t][s] *
+ * down[e] (silu(gate[e] x[t]) * (up[e] x[t])), e = idx[t][s]; s in ascending
+ * order, skipping experts outside [0, num_matrices).  gate_up is gated with
+ * outputs == down's cols, both with the same num_matrices; x and y
+ * [num_tokens][gate_up cols / down rows] contiguous of `dtype`, idx and
+ * weights [num_tokens][top_k] as moe_route_device writes them.
+ * num_tokens * top_k <= 512.  The hidden activations are kept in fp32 and
+ * enter the down product exactly. */
+int moe_w4_experts_device(MoeW4* gate_up, MoeW4* down, const void* x, int32_t dtype,
+                          int32_t num_tokens, int32_t top_k, const int32_t* idx,
+                          const float* weights, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
