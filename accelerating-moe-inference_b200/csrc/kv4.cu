@@ -3,9 +3,11 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "dtype.cuh"
 #include "kv4.cuh"
+#include "mma.cuh"
 #include "moe_internal.h"
 
 namespace moe {
@@ -274,65 +276,592 @@ struct AttendArgs {
     const int* q_offset;
     void* out;
     float* lse;
+    float* part;      // [2 * grid][rows of a tile][D + 2]: unnormalised outputs, then m and l
+    int* counter;     // [grid], zero between launches
     int tokens, H, Hkv, R, W, bs, nb, window;
     float scale;
+    bool vec;         // q rows can be read 16 bytes at a time
 };
 
-// One warp per (query token, head): the keys one after the other, each lane
-// owning 8 dims of every 256.
-template <class T, int D> __global__ void __launch_bounds__(128) attend_kernel(AttendArgs a) {
-    constexpr int kLanes = D / 8, G = D / 64;
-    const int lane = threadIdx.x & 31;
-    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int token = (int)(w / a.H), head = (int)(w % a.H);
-    if (token >= a.tokens) return;
-    int lo = 0, hi = a.R;   // the first r with q_offset[r + 1] > token, or R
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_offset[mid + 1] > token) hi = mid;
-        else lo = mid + 1;
+constexpr int kAttendWarps = 4;
+constexpr int kAttendStages = 4;
+constexpr int kAttendCtasPerSm = 4;
+constexpr int kAttendItemCost = 8;    // what an item costs beside its granules, in granules
+constexpr int kAttendMinUnits = 16;
+constexpr int kAttendWhole = 8;       // items of up to so many granules are not cut: joining costs more
+
+// What one request asks for: its queries [q0, q0 + nq), cut length, the
+// 16-token granules [lo, lo + n) that any of its queries may see, its items
+// and their cost.
+struct Request {
+    int q0, nq, len, lo, n, tiles, items;
+    long long units;
+};
+
+template <int kRows> __device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
+    Request q;
+    q.q0 = min(max(a.q_offset[r], 0), a.tokens);
+    q.nq = min(max(a.q_offset[r + 1], q.q0), a.tokens) - q.q0;
+    q.len = (int)min((long long)max(a.kv_len[r], 0), (long long)a.W * a.bs);
+    q.lo = a.window > 0 ? max(0, q.len - q.nq - a.window + 1) >> 4 : 0;
+    q.n = max(1, (int)(((long long)q.len + 15) >> 4) - q.lo);
+    const int rows_per_head = q.nq * (a.H / a.Hkv);
+    q.tiles = (rows_per_head + kRows - 1) / kRows;
+    q.items = a.Hkv * q.tiles;
+    q.units = (long long)q.items * (q.n + kAttendItemCost);
+    return q;
+}
+
+// The code pair at the nibbles `mask` names, as an operand.  As it stands it is
+// a pair of subnormals (c 2^-24, or c 2^-20 from the higher nibble of a byte):
+// exact, but the tensor core aligns a subnormal's products by its exponent
+// field, 2^3 to 2^10 above its value, and drops that much of the sum's low end
+// (measured: 5e-6 of the result's norm).  kNormal: made normal by one exact
+// multiplication by 2^14.
+template <bool kNormal> __device__ __forceinline__ uint32_t codes(uint32_t word, uint32_t mask) {
+    uint32_t v = word & mask;
+    if constexpr (kNormal) {
+        const __half2 k = __float2half2_rn(16384.0f);
+        const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), k);
+        v = *reinterpret_cast<const uint32_t*>(&r);
     }
-    if (lo == a.R || token < a.q_offset[lo]) return;
-    const int r = lo;
-    const int len = (int)min((long long)max(a.kv_len[r], 0), (long long)a.W * a.bs);
-    const int pos = len - min(a.q_offset[r + 1], a.tokens) + token;
-    const int kvh = head / (a.H / a.Hkv);
-    const int m = lane % kLanes, g = m >> 3;
-    float q[8], o[8];
-    const T* qp = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride + m * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        q[e] = to_f32(qp[e]) * a.scale;
-        o[e] = 0.0f;
+    return v;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Attention over the cache, one pass, the work split evenly over the blocks.
+//
+// Work: an item is (request, key/value head, tile of query rows); its units are
+// kAttendItemCost for what every item costs, then its 16-token granules.  Block
+// b takes the units [b * chunk, (b + 1) * chunk) of all items in order, so
+// ragged lengths cost no idle blocks and no length is read by the host.  Short
+// items stay whole, with the block that has their first unit.  An item that lies in several
+// blocks leaves partial (max, sum, output) rows; the block that finishes last
+// merges them in order of their place, so the result does not depend on the
+// order of arrival.
+//
+// A warp takes every fourth granule of its block's run and keeps four of them
+// in flight by asynchronous copies into its own ring; no warp waits for
+// another before the run ends.
+//
+// Products: m16n8k16 with the cache as A (16 tokens, then 16 dims of the
+// transposed values) and the query rows as the 8 columns of B, so that few
+// rows (a decode step's heads of one group) fill the product; the
+// probabilities of 16 tokens x 8 rows become the second product's B by an 8x8
+// transposition between the lanes.  A 4-bit code in the low bits of a float16
+// word is the subnormal c 2^-24 (or c 2^-20 four bits higher), so a code pair
+// becomes an operand by one AND, exactly (fp32: by one AND and one
+// multiplication, see codes()).  The scale and minimum of a key stand outside
+// its product,
+//   q . k = s (q . c) + m sum(q),
+// those of a value go into the probabilities before the second product,
+//   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t m_t.
+// fp32 queries take two float16 planes, hi and (x - hi) 2^11, as neighbouring
+// columns of the same product (22 bits); so do their probabilities.
+// NT: column tiles of 8.
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_kernel(AttendArgs a) {
+    constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
+    constexpr int kRows = 8 * NT / kPlanes;    // query rows of a tile
+    constexpr int kE = 2 / kPlanes;            // rows per lane and column tile
+    constexpr int kR = kE * NT;                // rows per lane
+    constexpr int G = D / 64;
+    constexpr int kGran = kv4_granule(D);
+    constexpr int kPitch = D + 4;              // floats per output row in shared memory
+    constexpr int kThreads = kAttendWarps * 32;
+    constexpr float kLo = 1.0f / 2048.0f;      // weight of the low plane
+    constexpr bool kNormal = kPlanes == 2;     // fp32 results need the whole of their sums
+    constexpr float kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
+    constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
+    static_assert((kRows * kPitch + 2 * kRows) * 4 <= kAttendStages * kGran, "a warp's result fits its ring");
+    extern __shared__ __align__(16) uint8_t attend_smem[];
+    __shared__ long long scan_buf[33];
+    __shared__ long long start_unit;
+    __shared__ int start_r, is_last;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    const int Gh = a.H / a.Hkv;
+    uint8_t* ring = attend_smem + warp * kAttendStages * kGran;
+    const uint32_t ring_u = smem_u32(ring);
+
+    // The block's share of the units, and the request its first one lies in.
+    const int per = (a.R + kThreads - 1) / kThreads;
+    const int r0 = min(a.R, (int)threadIdx.x * per), r1 = min(a.R, r0 + per);
+    long long mine = 0, total;
+    for (int r = r0; r < r1; ++r) mine += request_of<kRows>(a, r).units;
+    long long base = block_scan(mine, scan_buf, &total);
+    const long long chunk = max((total + gridDim.x - 1) / gridDim.x, (long long)kAttendMinUnits);
+    const long long u0 = blockIdx.x * chunk;
+    if (u0 >= total) return;
+    if (u0 >= base && u0 < base + mine) {
+        for (int r = r0; r < r1; ++r) {
+            const long long n = request_of<kRows>(a, r).units;
+            if (u0 < base + n) {
+                start_r = r;
+                start_unit = u0 - base;
+                break;
+            }
+            base += n;
+        }
     }
-    float mx = -INFINITY, sum = 0.0f;
-    for (int t = a.window > 0 ? max(0, pos - a.window + 1) : 0; t <= pos; ++t) {
-        const int page = a.table[(size_t)r * a.W + t / a.bs];
-        if (page < 0 || page >= a.nb) continue;
-        const int off = t % a.bs, tt = off & 15;
-        const uint8_t* gran = a.cache + (((long long)page * a.Hkv + kvh) * (a.bs >> 4) + (off >> 4)) * kv4_granule(D);
-        const uint32_t kw = *reinterpret_cast<const uint32_t*>(gran + kv4_k_word<D>(tt, m));
-        const uint32_t vw = *reinterpret_cast<const uint32_t*>(gran + kv4_v_word<D>(tt, m));
-        const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(gran + 16 * D + tt * G * 4 + g * 4));
-        const float2 vp = __half22float2(*reinterpret_cast<const __half2*>(gran + 16 * D + (16 + tt) * G * 4 + g * 4));
-        float x = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x += q[e] * fmaf(kp.x, (float)((kw >> (4 * e)) & 15), kp.y);
-#pragma unroll
-        for (int s = 1; s < kLanes; s <<= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-        const float next = fmaxf(mx, x);
-        const float keep = next == -INFINITY ? 1.0f : expf(mx - next), p = next == -INFINITY ? 0.0f : expf(x - next);
-        mx = next;
-        sum = sum * keep + p;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = o[e] * keep + p * fmaf(vp.x, (float)((vw >> (4 * e)) & 15), vp.y);
+    __syncthreads();
+    int r = start_r;
+    Request rq = request_of<kRows>(a, r);
+    int item = (int)(start_unit / (rq.n + kAttendItemCost));
+    int skip = (int)(start_unit % (rq.n + kAttendItemCost));   // units of it that lie in earlier blocks
+    long long left = min(total - u0, chunk);
+    if (skip > 0 && rq.n <= kAttendWhole) {   // the block with its first unit has all of it
+        left -= rq.n + kAttendItemCost - skip;
+        ++item;
+        skip = 0;
     }
-    if (lane < kLanes) {
-        T* op = static_cast<T*>(a.out) + ((long long)token * a.H + head) * D + m * 8;
+    const int page_grans = a.bs >> 4;                       // granules of a head in a page
+    const long long page_step = (long long)a.Hkv * page_grans;
+
+    while (left > 0) {
+        if (item == rq.items) {
+            rq = request_of<kRows>(a, ++r);   // units are left, so there is one
+            item = 0;
+            continue;
+        }
+        const int length = rq.n + kAttendItemCost;
+        const int count = rq.n <= kAttendWhole ? length : (int)min((long long)(length - skip), left);
+        const int first = max(0, skip - kAttendItemCost), last = max(0, skip + count - kAttendItemCost);
+        const long long item_u = u0 + min(total - u0, chunk) - left - skip;   // its first unit
+        const int head = item / rq.tiles, tile = item % rq.tiles;
+        ++item;
+        skip = 0;
+        left -= count;
+        if (last == 0) break;                 // its granules all lie in later blocks
+        const int rows = min(kRows, rq.nq * Gh - tile * kRows);
+        // Positions of the tile's first and last row, and the granules they see.
+        const int base_pos = rq.len - rq.nq;
+        const int pos_lo = base_pos + tile * kRows / Gh, pos_hi = base_pos + (tile * kRows + rows - 1) / Gh;
+        int ga = rq.lo + first, gb = rq.lo + last;
+        if (a.window > 0) ga = max(ga, max(0, pos_lo - a.window + 1) >> 4);
+        gb = min(gb, (pos_hi >> 4) + 1);       // pos_hi < 0: none
+
+        // The granule the next copy takes: its page's column and place there.
+        const int* table = a.table + (size_t)r * a.W;
+        int next = ga + warp, col = next / page_grans, sub = next % page_grans;
+        const uint8_t* head_base = a.cache + (long long)head * page_grans * kGran;
+        int page = next < gb ? table[col] : -1;
+        unsigned valid = 0;    // per stage: the granule's page lies in the pool
+        auto issue = [&](int stage) {
+            const bool in = page >= 0 && page < a.nb;       // also false past the run's end
+            valid = (valid & ~(1u << stage)) | ((unsigned)in << stage);
+            if (in) {
+                const uint8_t* src = head_base + (page * page_step + sub) * kGran + lane * 16;
+                const uint32_t dst = ring_u + stage * kGran + lane * 16;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) op[e] = from_f32<T>(sum == 0.0f ? 0.0f : o[e] / sum);   // a NaN stays one
+                for (int c = 0; c < kGran / 512; ++c) copy16_async(dst + c * 512, src + c * 512);
+                if (kGran % 512 && lane < kGran % 512 / 16) copy16_async(dst + kGran / 512 * 512, src + kGran / 512 * 512);
+            }
+            copy_commit();
+            next += kAttendWarps;
+            sub += kAttendWarps;
+            if (sub >= page_grans) {
+                const int pages = page_grans >= kAttendWarps ? 1 : sub / page_grans;
+                sub -= pages * page_grans;
+                col += pages;
+                page = next < gb ? table[col] : -1;
+            } else if (next >= gb) {
+                page = -1;
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < kAttendStages - 1; ++s) issue(s);
+
+        // The query fragments: rows scaled by a power of two to below 2^11,
+        // dims of even nibbles another 16 up to match their codes' 2^-24.
+        uint32_t qb[NT][D / 16][2];
+        float qs[kR][G], rowf[kR];
+        int row_pos[kR];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int local = (n * 8 + g) / kPlanes, row = tile * kRows + local;
+            const bool on = local < rows;
+            float x[2 * G][8];
+            float mx = 0.0f;
+            const T* qp = static_cast<const T*>(a.q) + (on ? (rq.q0 + row / Gh) * a.q_token_stride +
+                                                              (head * Gh + row % Gh) * a.q_head_stride : 0);
+#pragma unroll
+            for (int w = 0; w < 2 * G; ++w) {
+                const T* p = qp + 64 * (w >> 1) + 16 * j + 8 * (w & 1);
+                if (on && a.vec) {
+                    load8<T, true>(p, x[w]);
+                } else if (on) {
+                    load8<T, false>(p, x[w]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[w][e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[w][e]));
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // Exponent of the largest, kept where 2^(10 - e) is a normal number.
+            const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
+            const float up = __uint_as_float((264 - e) << 23);              // 2^(10 - (e - 127))
+            const float f = a.scale * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kUnit;
+            float sum[G];
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                sum[q] = 0.0f;
+#pragma unroll
+                for (int w = 2 * q; w < 2 * q + 2; ++w)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum[q] += x[w][k] *= up;
+                sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], 1);
+                sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], 2);
+                sum[q] *= 1.0f / kUnit;
+            }
+#pragma unroll
+            for (int w = 0; w < 2 * G; ++w)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float k16 = k & 1 ? 1.0f : 16.0f;
+                    const float p0 = x[w][k] * k16, p1 = x[w][k + 4] * k16;
+                    uint32_t v = half2_bits(p0, p1);
+                    if constexpr (kPlanes == 2) {
+                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                        if (g & 1) v = half2_bits((p0 - b.x) * 2048.0f, (p1 - b.y) * 2048.0f);
+                    }
+                    qb[n][2 * w + (k >> 1)][k & 1] = v;
+                }
+            // What a row's scores need, to the lanes that hold them.
+#pragma unroll
+            for (int i = 0; i < kE; ++i) {
+                const int src = 8 * j + 4 * i;   // lane of column 2 j + i (fp32: 2 j)
+                rowf[n * kE + i] = __shfl_sync(0xffffffffu, f, src);
+#pragma unroll
+                for (int q = 0; q < G; ++q) qs[n * kE + i][q] = __shfl_sync(0xffffffffu, sum[q], src);
+                row_pos[n * kE + i] = base_pos + (tile * kRows + (n * 8 + 2 * j) / kPlanes + i) / Gh;
+            }
+        }
+
+        // Transposed outputs: lane's rows, dims 64 q + 8 g + 2 i (c0, c1) and + 1 (c2, c3).
+        float o[NT][G][4][4], m[kR], l[kR], w0[kR][G];
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < G; ++q) w0[i][q] = 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < G; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[n][q][i][c] = 0.0f;
+
+        int stage = 0;
+        for (int gi = ga + warp; gi < gb; gi += kAttendWarps) {
+            copy_wait<kAttendStages - 2>();
+            __syncwarp();
+            const uint32_t st = ring_u + stage * kGran;
+            if ((valid >> stage) & 1) {
+                // Scores x[row][h] of the lane's rows and tokens g + 8 h.
+                float x[kR][2];
+                {
+                    uint32_t kw[2][2 * G];
+                    float acc[NT][G][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if constexpr (G == 2) {
+                            const uint4 v = lds128(st + h * 512 + lane * 16);
+                            kw[h][0] = v.x, kw[h][1] = v.y, kw[h][2] = v.z, kw[h][3] = v.w;
+                        } else {
+                            const uint2 v = lds64(st + h * 256 + lane * 8);
+                            kw[h][0] = v.x, kw[h][1] = v.y;
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < G; ++q) {
+#pragma unroll
+                        for (int w = 2 * q; w < 2 * q + 2; ++w)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const uint32_t lo = kw[0][w] >> (8 * half), hi = kw[1][w] >> (8 * half);
+                                const uint32_t f[4] = {codes<kNormal>(lo, kEven), codes<kNormal>(hi, kEven),
+                                                       codes<kNormal>(lo, kOdd), codes<kNormal>(hi, kOdd)};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    if (w == 2 * q && half == 0) mma_f16_first(acc[n][q], f, qb[n][2 * w][0], qb[n][2 * w][1]);
+                                    else mma_f16(acc[n][q], f, qb[n][2 * w + half][0], qb[n][2 * w + half][1]);
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t kp[G];
+                        const uint32_t at = st + 16 * D + (g + 8 * h) * G * 4;
+                        if constexpr (G == 2) {
+                            const uint2 v = lds64(at);
+                            kp[0] = v.x, kp[1] = v.y;
+                        } else {
+                            kp[0] = lds32(at);
+                        }
+#pragma unroll
+                        for (int i = 0; i < kR; ++i) x[i][h] = 0.0f;
+#pragma unroll
+                        for (int q = 0; q < G; ++q) {
+                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
+#pragma unroll
+                            for (int i = 0; i < kR; ++i) {
+                                const float (&t)[4] = acc[i / kE][q];
+                                const float d = kPlanes == 2 ? fmaf(t[2 * h + 1], kLo, t[2 * h]) : t[2 * h + i % kE];
+                                x[i][h] = fmaf(p.x, d, fmaf(p.y, qs[i][q], x[i][h]));
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < kR; ++i) x[i][h] *= rowf[i];
+                    }
+                }
+                const int t0 = gi << 4;
+                const bool edge = t0 + 15 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
+                unsigned hide = 0;
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < kR; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int t = t0 + 8 * h + g;
+                            if (t > row_pos[i] || (a.window > 0 && t <= row_pos[i] - a.window)) {
+                                x[i][h] = -INFINITY;
+                                hide |= 1u << (2 * i + h);
+                            }
+                        }
+                }
+                // The reference point m of a row's exponentials moves only when a
+                // score lies more than 2 above it: p stays below 4, and with a
+                // scale of at most 8736 p s stays a float16.
+                bool above = false;
+#pragma unroll
+                for (int i = 0; i < kR; ++i) above |= fmaxf(x[i][0], x[i][1]) > m[i] + 2.0f;
+                if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                    for (int i = 0; i < kR; ++i) {
+                        float top = fmaxf(x[i][0], x[i][1]);
+#pragma unroll
+                        for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                        const float keep = top > m[i] ? exp2_approx(m[i] - top) : 1.0f;
+                        m[i] = fmaxf(m[i], top);
+                        l[i] *= keep;
+#pragma unroll
+                        for (int q = 0; q < G; ++q) {
+                            w0[i][q] *= keep;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                float (&t)[4] = o[i / kE][q][k];
+                                t[i % kE] *= keep;
+                                t[2 + i % kE] *= keep;
+                                if constexpr (kPlanes == 2) {
+                                    t[1] *= keep;
+                                    t[3] *= keep;
+                                }
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kR; ++i) {
+                    const float off = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        x[i][h] = exp2_approx(x[i][h] - off);
+                        l[i] += x[i][h];
+                    }
+                }
+                // The second product's B: row g, tokens 2 j + 8 h, + 1.
+                uint32_t pb[NT][G][2];
+                auto weigh = [&](auto at_edge) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t vp[G];
+                        const uint32_t at = st + 16 * D + 64 * G + (g + 8 * h) * G * 4;
+                        if constexpr (G == 2) {
+                            const uint2 v = lds64(at);
+                            vp[0] = v.x, vp[1] = v.y;
+                        } else {
+                            vp[0] = lds32(at);
+                        }
+#pragma unroll
+                        for (int q = 0; q < G; ++q) {
+                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&vp[q]));
+                            float v[kR];
+#pragma unroll
+                            for (int i = 0; i < kR; ++i) {
+                                v[i] = x[i][h] * p.x;
+                                if constexpr (at_edge) {   // a hidden token's params may be anything
+                                    const bool hidden = hide >> (2 * i + h) & 1;
+                                    v[i] = hidden ? 0.0f : v[i];
+                                    w0[i][q] += hidden ? 0.0f : x[i][h] * p.y;
+                                } else {
+                                    w0[i][q] = fmaf(x[i][h], p.y, w0[i][q]);
+                                }
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                uint32_t b;
+                                if constexpr (kPlanes == 2) {
+                                    const float hi = __half2float(__float2half_rn(v[n]));
+                                    b = half2_bits(hi, (v[n] - hi) * 2048.0f);
+                                } else {
+                                    b = half2_bits(v[2 * n], v[2 * n + 1]);
+                                }
+                                pb[n][q][h] = transpose8x8(b);
+                            }
+                        }
+                    }
+                };
+                if (edge) weigh(std::true_type{});
+                else weigh(std::false_type{});
+                // Values: lane's tokens 2 j, 2 j + 1 of each half, dims 64 q + 8 g + nibble.
+                uint32_t vw[2][2][G];   // [half][token][group]
+                if constexpr (G == 2) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4 v = lds128(st + 8 * D + h * 512 + lane * 16);
+                        vw[h][0][0] = v.x, vw[h][0][1] = v.y, vw[h][1][0] = v.z, vw[h][1][1] = v.w;
+                    }
+                } else {
+                    const uint4 v = lds128(st + 8 * D + lane * 16);
+                    vw[0][0][0] = v.x, vw[0][1][0] = v.y, vw[1][0][0] = v.z, vw[1][1][0] = v.w;
+                }
+#pragma unroll
+                for (int q = 0; q < G; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {   // nibbles 2 i (rows g) and 2 i + 1 (rows g + 8)
+                        const uint32_t sel = i >> 1 ? 0x7632 : 0x5410;
+                        const uint32_t b0 = __byte_perm(vw[0][0][q], vw[0][1][q], sel) >> (8 * (i & 1));
+                        const uint32_t b1 = __byte_perm(vw[1][0][q], vw[1][1][q], sel) >> (8 * (i & 1));
+                        const uint32_t f[4] = {codes<kNormal>(b0, kEven), codes<kNormal>(b0, kOdd),
+                                               codes<kNormal>(b1, kEven), codes<kNormal>(b1, kOdd)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_f16(o[n][q][i], f, pb[n][q][0], pb[n][q][1]);
+                    }
+            }
+            __syncwarp();
+            issue((stage + kAttendStages - 1) % kAttendStages);
+            stage = (stage + 1) % kAttendStages;
+        }
+        copy_wait<0>();
+        __syncwarp();
+
+        // The warp's rows into its ring's place: output, then m and l.
+        float* res = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int i = 0; i < kR; ++i) {
+            const int row = (i / kE * 8 + 2 * j) / kPlanes + i % kE;
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], k);
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                float z = w0[i][q];
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float (&t)[4] = o[i / kE][q][k];
+                    const float d0 = kPlanes == 2 ? fmaf(t[1], kLo, t[0]) : t[i % kE];
+                    const float d1 = kPlanes == 2 ? fmaf(t[3], kLo, t[2]) : t[2 + i % kE];
+                    v[2 * k] = fmaf(d0, 16.0f * kUnit, z);
+                    v[2 * k + 1] = fmaf(d1, kUnit, z);
+                }
+                float* to = res + row * kPitch + 64 * q + 8 * g;
+                *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+            if (g == 0) {
+                res[kRows * kPitch + 2 * row] = m[i];
+                res[kRows * kPitch + 2 * row + 1] = l[i];
+            }
+        }
+        __syncthreads();
+
+        const bool whole = first == 0 && last == rq.n;
+        float* part = a.part + (2 * (long long)blockIdx.x + (first == 0 ? 1 : 0)) * kRows * (D + 2);
+        constexpr int kWarpFloats = kAttendStages * kGran / 4;
+        auto write = [&](int row, int d, float4 v, float mm, float ll) {
+            const int rr = tile * kRows + row;
+            const long long at = (long long)(rq.q0 + rr / Gh) * a.H + head * Gh + rr % Gh;
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;    // no key seen: 0; a NaN stays one
+            T* op = static_cast<T*>(a.out) + at * D + d;
+            T t[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(t);
+            else *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(t);
+            if (a.lse && d == 0)
+                a.lse[at] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+        };
+        for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+            const int row = i / (D / 4), d = i % (D / 4) * 4;
+            const float* w = reinterpret_cast<const float*>(attend_smem);
+            float mm = -INFINITY, ll = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kAttendWarps; ++k) mm = fmaxf(mm, w[k * kWarpFloats + kRows * kPitch + 2 * row]);
+            const float off = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+            for (int k = 0; k < kAttendWarps; ++k) {
+                const float f = exp2_approx(w[k * kWarpFloats + kRows * kPitch + 2 * row] - off);
+                ll = fmaf(w[k * kWarpFloats + kRows * kPitch + 2 * row + 1], f, ll);
+                const float4 t = *reinterpret_cast<const float4*>(w + k * kWarpFloats + row * kPitch + d);
+                v.x = fmaf(t.x, f, v.x), v.y = fmaf(t.y, f, v.y), v.z = fmaf(t.z, f, v.z), v.w = fmaf(t.w, f, v.w);
+            }
+            if (whole) {
+                write(row, d, v, mm, ll);
+            } else {
+                *reinterpret_cast<float2*>(part + row * (D + 2) + d) = make_float2(v.x, v.y);
+                *reinterpret_cast<float2*>(part + row * (D + 2) + d + 2) = make_float2(v.z, v.w);
+                if (d == 0) *reinterpret_cast<float2*>(part + row * (D + 2) + D) = make_float2(mm, ll);
+            }
+        }
+        if (!whole) {
+            // The blocks that hold its granules.
+            const long long c0 = (item_u + kAttendItemCost) / chunk, c1 = (item_u + length - 1) / chunk;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) is_last = atomicAdd(a.counter + c0, 1) == (int)(c1 - c0);
+            __syncthreads();
+            if (is_last) {
+                __threadfence();
+                if (threadIdx.x == 0) a.counter[c0] = 0;
+                // The item begins in block c0 (its second part) and covers the
+                // first part of every later one.
+                const float* p0 = a.part + (2 * c0 + 1) * kRows * (D + 2);
+                const long long step = 2ll * kRows * (D + 2);
+                for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+                    const int row = i / (D / 4), d = i % (D / 4) * 4;
+                    float mm = -INFINITY, ll = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (long long c = c0; c <= c1; ++c) {
+                        const float* p = p0 + (c - c0) * step - (c > c0 ? kRows * (D + 2) : 0) + row * (D + 2);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + D));
+                        const float2 x0 = __ldcg(reinterpret_cast<const float2*>(p + d));
+                        const float2 x1 = __ldcg(reinterpret_cast<const float2*>(p + d + 2));
+                        const float big = fmaxf(mm, ml.x), off = big == -INFINITY ? 0.0f : big;
+                        const float f0 = exp2_approx(mm - off), f1 = exp2_approx(ml.x - off);
+                        mm = big;
+                        ll = fmaf(ll, f0, ml.y * f1);
+                        v.x = fmaf(v.x, f0, x0.x * f1), v.y = fmaf(v.y, f0, x0.y * f1);
+                        v.z = fmaf(v.z, f0, x1.x * f1), v.w = fmaf(v.w, f0, x1.y * f1);
+                    }
+                    write(row, d, v, mm, ll);
+                }
+            }
+        }
+        __syncthreads();   // the rings and is_last are free again
     }
-    if (lane == 0 && a.lse) a.lse[(long long)token * a.H + head] = sum == 0.0f ? -INFINITY : mx + logf(sum);
 }
 
 }  // namespace
@@ -340,7 +869,10 @@ template <class T, int D> __global__ void __launch_bounds__(128) attend_kernel(A
 
 struct MoeKv4 {
     MoeKv4Config cfg;
-    int sm_count = 148;
+    int sms = 0;
+    float* part = nullptr;     // attention: partial rows of items that several blocks share
+    int* counter = nullptr;
+    size_t bytes = 0;
 };
 
 using namespace moe;
@@ -369,9 +901,9 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
         if (cfg->block_tokens < 16 || cfg->block_tokens > 1024 || cfg->block_tokens % 16)
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: block_tokens must be a multiple of 16, 16..1024");
         if (cfg->num_blocks < 1 || cfg->table_width < 1 ||
-            (long long)cfg->table_width * cfg->block_tokens > 0x7fffffffll)
+            (long long)cfg->table_width * cfg->block_tokens > (1 << 30))
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: need num_blocks >= 1, table_width >= 1 and "
-                                                 "table_width * block_tokens within 31 bits");
+                                                 "table_width * block_tokens <= 2^30");
         if (cfg->max_requests < 1 || cfg->max_requests > 8192)
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: max_requests must be 1..8192");
         int ndev = 0;
@@ -390,13 +922,33 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
             return report_error(MOE_ERR_UNSUPPORTED, "libmoe_b200 is built for sm_100a (B200) only");
         auto* h = new MoeKv4;
         h->cfg = *cfg;
-        h->sm_count = sms;
+        h->sms = sms;
+        const size_t grid = (size_t)sms * kAttendCtasPerSm;
+        const size_t part = grid * 2 * 16 * (cfg->head_dim + 2) * sizeof(float);
+        const size_t counter = grid * sizeof(int);
+        e = cudaMalloc(&h->part, part);
+        if (e == cudaSuccess) e = cudaMalloc(&h->counter, counter);
+        if (e == cudaSuccess) e = cudaMemset(h->counter, 0, counter);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            moe_kv4_destroy(h);
+            return report_error(e == cudaErrorMemoryAllocation ? MOE_ERR_OOM : MOE_ERR_CUDA,
+                                std::string("moe_kv4_create: ") + cudaGetErrorString(e));
+        }
+        h->bytes = part + counter;
         *out = h;
         return MOE_OK;
     });
 }
 
-void moe_kv4_destroy(MoeKv4* h) { delete h; }
+void moe_kv4_destroy(MoeKv4* h) {
+    if (!h) return;
+    OnDevice on(h->cfg.device);
+    cudaFree(h->part);
+    cudaFree(h->counter);
+    delete h;
+}
 
 size_t moe_kv4_cache_bytes(const MoeKv4* h) {
     if (!h) return 0;
@@ -404,7 +956,7 @@ size_t moe_kv4_cache_bytes(const MoeKv4* h) {
     return (size_t)c.num_blocks * c.num_kv_heads * (c.block_tokens / 16) * kv4_granule(c.head_dim);
 }
 
-size_t moe_kv4_device_bytes(const MoeKv4* h) { (void)h; return 0; }
+size_t moe_kv4_device_bytes(const MoeKv4* h) { return h ? h->bytes : 0; }
 
 int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new_len, int32_t R, int32_t* free_ring,
                         const int32_t* ring_state, int32_t* block_table, int32_t* kv_len, int32_t* q_offset,
@@ -446,10 +998,17 @@ template <class T> cudaError_t append_dim(const AppendArgs& a, int D, bool vec, 
     return D == 64 ? append_typed<T, 64>(a, vec, s) : append_typed<T, 128>(a, vec, s);
 }
 
-template <class T> cudaError_t attend_dim(const AttendArgs& a, int D, cudaStream_t s) {
-    const unsigned grid = (unsigned)(((long long)a.tokens * a.H + 3) / 4);
-    return D == 64 ? launch(attend_kernel<T, 64>, grid, 128, 0, s, false, a)
-                   : launch(attend_kernel<T, 128>, grid, 128, 0, s, false, a);
+template <class T, int D> cudaError_t attend_tiles(const AttendArgs& a, int sms, cudaStream_t s) {
+    const dim3 block(kAttendWarps * 32);
+    const size_t smem = (size_t)kAttendWarps * kAttendStages * kv4_granule(D);
+    // Columns that a request's queries of one key/value head need on average.
+    const long long columns = (long long)(a.H / a.Hkv) * ((a.tokens + a.R - 1) / a.R) * (sizeof(T) == 4 ? 2 : 1);
+    return columns <= 8 ? launch(attend_kernel<T, D, 1>, sms * kAttendCtasPerSm, block, smem, s, false, a)
+                        : launch(attend_kernel<T, D, 2>, sms * 2, block, smem, s, false, a);
+}
+
+template <class T> cudaError_t attend_dim(const AttendArgs& a, int D, int sms, cudaStream_t s) {
+    return D == 64 ? attend_tiles<T, 64>(a, sms, s) : attend_tiles<T, 128>(a, sms, s);
 }
 
 }  // namespace
@@ -504,7 +1063,7 @@ int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_
         if (R < 1 || R > c.max_requests || tokens < 0 || window < 0 || !std::isfinite(scale))
             return report_error(MOE_ERR_INVALID, "moe_kv4_attention_device: need 1 <= num_requests <= max_requests, "
                                                  "tokens >= 0, window >= 0 and a finite scale");
-        if ((long long)tokens * num_heads > 0x7fffffffll)
+        if ((long long)tokens * num_heads > 0x7fffffffll || tokens > (1 << 30))
             return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_attention_device: too many tokens for one call");
         if (tokens == 0) return MOE_OK;
         if (!cache || !q || !block_table || !kv_len || !q_offset || !out)
@@ -515,12 +1074,14 @@ int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_
         OnDevice on(c.device);
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_attention_device: cannot select the device");
         AttendArgs a{static_cast<const uint8_t*>(cache), q, q_token_stride, q_head_stride, block_table, kv_len,
-                     q_offset, out, lse, tokens, num_heads, c.num_kv_heads, R, c.table_width, c.block_tokens,
-                     c.num_blocks, window, scale};
+                     q_offset, out, lse, h->part, h->counter, tokens, num_heads, c.num_kv_heads, R, c.table_width, c.block_tokens,
+                     c.num_blocks, (long long)window >= (long long)c.table_width * c.block_tokens ? 0 : window, scale, false};
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
-        cudaError_t e = dtype == MOE_DTYPE_F32    ? attend_dim<float>(a, c.head_dim, s)
-                        : dtype == MOE_DTYPE_BF16 ? attend_dim<__nv_bfloat16>(a, c.head_dim, s)
-                                                  : attend_dim<__half>(a, c.head_dim, s);
+        const int64_t es = (int64_t)dtype_bytes(dtype);
+        a.vec = aligned16(q) && q_token_stride * es % 16 == 0 && q_head_stride * es % 16 == 0;
+        cudaError_t e = dtype == MOE_DTYPE_F32    ? attend_dim<float>(a, c.head_dim, h->sms, s)
+                        : dtype == MOE_DTYPE_BF16 ? attend_dim<__nv_bfloat16>(a, c.head_dim, h->sms, s)
+                                                  : attend_dim<__half>(a, c.head_dim, h->sms, s);
         return launch_status(e, "moe_kv4_attention_device");
     });
 }

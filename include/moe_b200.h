@@ -528,7 +528,7 @@ typedef struct MoeKv4Config {
     int32_t head_dim;      /* 64 or 128 */
     int32_t block_tokens;  /* tokens per page: a multiple of 16, at most 1024 */
     int32_t num_blocks;    /* pages of the pool */
-    int32_t table_width;   /* block-table entries per request */
+    int32_t table_width;   /* block-table entries per request; table_width * block_tokens <= 2^30 */
     int32_t max_requests;  /* requests per call, 1..8192 */
     int32_t device;
     int32_t reserved[5];
