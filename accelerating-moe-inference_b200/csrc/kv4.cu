@@ -267,6 +267,21 @@ template <class T, int D, bool kVec> __global__ void __launch_bounds__(256) appe
 }
 
 // -------------------------------------------------------------- attention
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^s >= d the
+// smallest such power, q = floor(n m / 2^(31 + s)) for m = ceil(2^(31 + s) / d),
+// since n (m d - 2^(31 + s)) < 2^31 d <= 2^(31 + s).
+struct FastDiv {
+    unsigned long long mul;
+    int shift, d;
+    FastDiv() = default;
+    explicit FastDiv(int div) : d(div) {
+        shift = 31;
+        while ((1ll << (shift - 31)) < div) ++shift;
+        mul = ((1ull << shift) + div - 1) / div;
+    }
+    __device__ __forceinline__ int div(int n) const { return (int)((unsigned)n * mul >> shift); }
+};
+
 struct AttendArgs {
     const uint8_t* cache;
     const void* q;
@@ -281,13 +296,15 @@ struct AttendArgs {
     int tokens, H, Hkv, R, W, bs, nb, window;
     float scale;
     bool vec;         // q rows can be read 16 bytes at a time
+    FastDiv group;    // by H / Hkv
+    FastDiv page;     // by bs / 16
 };
 
 constexpr int kAttendWarps = 4;
-constexpr int kAttendStages = 4;
-constexpr int kAttendCtasPerSm = 4;
-constexpr int kAttendItemCost = 8;    // what an item costs beside its granules, in granules
-constexpr int kAttendMinUnits = 16;
+constexpr int kAttendStages = 3;      // granule pairs in flight per warp
+constexpr int kAttendCtasPerSm = 3;
+constexpr int kAttendItemCost = 16;   // what an item costs beside its granules, in granules (measured: 17)
+constexpr int kAttendMinUnits = 24;
 constexpr int kAttendWhole = 8;       // items of up to so many granules are not cut: joining costs more
 
 // What one request asks for: its queries [q0, q0 + nq), cut length, the
@@ -344,7 +361,7 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // merges them in order of their place, so the result does not depend on the
 // order of arrival.
 //
-// A warp takes every fourth granule of its block's run and keeps four of them
+// A warp takes every fourth pair of granules of its block's run and keeps three of them
 // in flight by asynchronous copies into its own ring; no warp waits for
 // another before the run ends.
 //
@@ -364,7 +381,7 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // columns of the same product (22 bits); so do their probabilities.
 // NT: column tiles of 8.
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm : 2) attend_kernel(AttendArgs a) {
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     constexpr int kRows = 8 * NT / kPlanes;    // query rows of a tile
     constexpr int kE = 2 / kPlanes;            // rows per lane and column tile
@@ -377,15 +394,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
     constexpr bool kNormal = kPlanes == 2;     // fp32 results need the whole of their sums
     constexpr float kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
-    static_assert((kRows * kPitch + 2 * kRows) * 4 <= kAttendStages * kGran, "a warp's result fits its ring");
+    constexpr int kStage = 2 * kGran;
+    static_assert((kRows * kPitch + 2 * kRows) * 4 <= kAttendStages * kStage, "a warp's result fits its ring");
     extern __shared__ __align__(16) uint8_t attend_smem[];
     __shared__ long long scan_buf[33];
     __shared__ long long start_unit;
-    __shared__ int start_r, is_last;
+    __shared__ int start_r, is_last, join_from, join_to;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
     const int Gh = a.H / a.Hkv;
-    uint8_t* ring = attend_smem + warp * kAttendStages * kGran;
+    uint8_t* ring = attend_smem + warp * kAttendStages * kStage;
     const uint32_t ring_u = smem_u32(ring);
 
     // The block's share of the units, and the request its first one lies in.
@@ -420,7 +438,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
         skip = 0;
     }
     const int page_grans = a.bs >> 4;                       // granules of a head in a page
-    const long long page_step = (long long)a.Hkv * page_grans;
+    const unsigned page_step = (unsigned)a.Hkv * page_grans;   // the granules of a cache are below 2^32 - 1
 
     while (left > 0) {
         if (item == rq.items) {
@@ -432,7 +450,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
         const int count = rq.n <= kAttendWhole ? length : (int)min((long long)(length - skip), left);
         const int first = max(0, skip - kAttendItemCost), last = max(0, skip + count - kAttendItemCost);
         const long long item_u = u0 + min(total - u0, chunk) - left - skip;   // its first unit
-        const int head = item / rq.tiles, tile = item % rq.tiles;
+        const int head = rq.tiles == 1 ? item : item / rq.tiles, tile = item - head * rq.tiles;
         ++item;
         skip = 0;
         left -= count;
@@ -440,37 +458,52 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
         const int rows = min(kRows, rq.nq * Gh - tile * kRows);
         // Positions of the tile's first and last row, and the granules they see.
         const int base_pos = rq.len - rq.nq;
-        const int pos_lo = base_pos + tile * kRows / Gh, pos_hi = base_pos + (tile * kRows + rows - 1) / Gh;
+        const int pos_lo = base_pos + a.group.div(tile * kRows);
+        const int pos_hi = base_pos + a.group.div(tile * kRows + rows - 1);
         int ga = rq.lo + first, gb = rq.lo + last;
         if (a.window > 0) ga = max(ga, max(0, pos_lo - a.window + 1) >> 4);
         gb = min(gb, (pos_hi >> 4) + 1);       // pos_hi < 0: none
 
-        // The granule the next copy takes: its page's column and place there.
+        // Where the warp's granules lie, 16 pairs at a time: lane i holds the
+        // place in the cache of the i-th one, kNone without one or where its
+        // page is outside the pool; `later` the next 32's, loaded ahead.
+        constexpr unsigned kNone = 0xffffffffu;
         const int* table = a.table + (size_t)r * a.W;
-        int next = ga + warp, col = next / page_grans, sub = next % page_grans;
-        const uint8_t* head_base = a.cache + (long long)head * page_grans * kGran;
-        int page = next < gb ? table[col] : -1;
-        unsigned valid = 0;    // per stage: the granule's page lies in the pool
+        const uint8_t* head_base = a.cache + (long long)head * page_grans * kGran + lane * 16;
+        int ahead = ga + 2 * warp + (lane >> 1) * (2 * kAttendWarps) + (lane & 1);
+        auto locate = [&]() {
+            unsigned at = kNone;
+            if (ahead < gb) {
+                const int col = a.page.div(ahead), page = table[col];
+                if (page >= 0 && page < a.nb) at = (unsigned)page * page_step + (unsigned)(ahead - col * page_grans);
+            }
+            ahead += 32 * kAttendWarps;
+            return at;
+        };
+        unsigned here = locate(), later = locate();
+        int pair = 0;
+        unsigned valid = 0;    // two bits per stage: there is such a granule
         auto issue = [&](int stage) {
-            const bool in = page >= 0 && page < a.nb;       // also false past the run's end
-            valid = (valid & ~(1u << stage)) | ((unsigned)in << stage);
-            if (in) {
-                const uint8_t* src = head_base + (page * page_step + sub) * kGran + lane * 16;
-                const uint32_t dst = ring_u + stage * kGran + lane * 16;
 #pragma unroll
-                for (int c = 0; c < kGran / 512; ++c) copy16_async(dst + c * 512, src + c * 512);
-                if (kGran % 512 && lane < kGran % 512 / 16) copy16_async(dst + kGran / 512 * 512, src + kGran / 512 * 512);
+            for (int k = 0; k < 2; ++k) {
+                const unsigned at = __shfl_sync(0xffffffffu, here, 2 * pair + k);
+                const unsigned bit = 1u << (2 * stage + k);
+                valid &= ~bit;
+                if (at != kNone) {
+                    valid |= bit;
+                    const uint8_t* src = head_base + (unsigned long long)at * kGran;
+                    const uint32_t dst = ring_u + stage * kStage + k * kGran + lane * 16;
+#pragma unroll
+                    for (int c = 0; c < kGran / 512; ++c) copy16_async(dst + c * 512, src + c * 512);
+                    if (kGran % 512 && lane < kGran % 512 / 16)
+                        copy16_async(dst + kGran / 512 * 512, src + kGran / 512 * 512);
+                }
             }
             copy_commit();
-            next += kAttendWarps;
-            sub += kAttendWarps;
-            if (sub >= page_grans) {
-                const int pages = page_grans >= kAttendWarps ? 1 : sub / page_grans;
-                sub -= pages * page_grans;
-                col += pages;
-                page = next < gb ? table[col] : -1;
-            } else if (next >= gb) {
-                page = -1;
+            if (++pair == 16) {
+                pair = 0;
+                here = later;
+                later = locate();
             }
         };
 #pragma unroll
@@ -487,8 +520,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
             const bool on = local < rows;
             float x[2 * G][8];
             float mx = 0.0f;
-            const T* qp = static_cast<const T*>(a.q) + (on ? (rq.q0 + row / Gh) * a.q_token_stride +
-                                                              (head * Gh + row % Gh) * a.q_head_stride : 0);
+            const int tok = a.group.div(row);
+            const T* qp = static_cast<const T*>(a.q) + (on ? (rq.q0 + tok) * a.q_token_stride +
+                                                              (head * Gh + row - tok * Gh) * a.q_head_stride : 0);
 #pragma unroll
             for (int w = 0; w < 2 * G; ++w) {
                 const T* p = qp + 64 * (w >> 1) + 16 * j + 8 * (w & 1);
@@ -507,8 +541,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             // Exponent of the largest, kept where 2^(10 - e) is a normal number.
             const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
-            const float up = __uint_as_float((264 - e) << 23);              // 2^(10 - (e - 127))
-            const float f = a.scale * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kUnit;
+            const float up = copysignf(__uint_as_float((264 - e) << 23), a.scale);   // +-2^(10 - (e - 127))
+            const float f = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kUnit, 1e-37f);
             float sum[G];
 #pragma unroll
             for (int q = 0; q < G; ++q) {
@@ -541,16 +575,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                 rowf[n * kE + i] = __shfl_sync(0xffffffffu, f, src);
 #pragma unroll
                 for (int q = 0; q < G; ++q) qs[n * kE + i][q] = __shfl_sync(0xffffffffu, sum[q], src);
-                row_pos[n * kE + i] = base_pos + (tile * kRows + (n * 8 + 2 * j) / kPlanes + i) / Gh;
+                row_pos[n * kE + i] = base_pos + a.group.div(tile * kRows + (n * 8 + 2 * j) / kPlanes + i);
             }
         }
 
         // Transposed outputs: lane's rows, dims 64 q + 8 g + 2 i (c0, c1) and + 1 (c2, c3).
-        float o[NT][G][4][4], m[kR], l[kR], w0[kR][G];
+        float o[NT][G][4][4], m[kR], l[kR], w0[kR][G], limit[kR], room[kR], off[kR];
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
+            m[i] = limit[i] = -INFINITY;
+            room[i] = 2.0f / rowf[i];
+            l[i] = off[i] = 0.0f;
 #pragma unroll
             for (int q = 0; q < G; ++q) w0[i][q] = 0.0f;
         }
@@ -564,14 +599,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                     for (int c = 0; c < 4; ++c) o[n][q][i][c] = 0.0f;
 
         int stage = 0;
-        for (int gi = ga + warp; gi < gb; gi += kAttendWarps) {
+        for (int gi = ga + 2 * warp; gi < gb; gi += 2 * kAttendWarps) {
             copy_wait<kAttendStages - 2>();
             __syncwarp();
-            const uint32_t st = ring_u + stage * kGran;
-            if ((valid >> stage) & 1) {
-                // Scores x[row][h] of the lane's rows and tokens g + 8 h.
-                float x[kR][2];
-                {
+            const uint32_t st0 = ring_u + stage * kStage;
+            const unsigned have = valid >> (2 * stage) & 3;
+            if (have) {
+                // Scores x[row][2 k + h] of the lane's rows and tokens 16 k + g + 8 h.
+                float x[kR][4];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t st = st0 + k * kGran;
                     uint32_t kw[2][2 * G];
                     float acc[NT][G][4];
 #pragma unroll
@@ -610,8 +648,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                         } else {
                             kp[0] = lds32(at);
                         }
-#pragma unroll
-                        for (int i = 0; i < kR; ++i) x[i][h] = 0.0f;
+                        float s[kR];
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
                             const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
@@ -619,42 +656,47 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                             for (int i = 0; i < kR; ++i) {
                                 const float (&t)[4] = acc[i / kE][q];
                                 const float d = kPlanes == 2 ? fmaf(t[2 * h + 1], kLo, t[2 * h]) : t[2 * h + i % kE];
-                                x[i][h] = fmaf(p.x, d, fmaf(p.y, qs[i][q], x[i][h]));
+                                s[i] = q == 0 ? p.y * qs[i][q] : fmaf(p.y, qs[i][q], s[i]);
+                                s[i] = fmaf(p.x, d, s[i]);
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < kR; ++i) x[i][h] *= rowf[i];
+                        for (int i = 0; i < kR; ++i) x[i][2 * k + h] = s[i];
                     }
                 }
                 const int t0 = gi << 4;
-                const bool edge = t0 + 15 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
+                const bool edge = have != 3 || t0 + 31 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
                 unsigned hide = 0;
                 if (edge) {
 #pragma unroll
                     for (int i = 0; i < kR; ++i)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int t = t0 + 8 * h + g;
-                            if (t > row_pos[i] || (a.window > 0 && t <= row_pos[i] - a.window)) {
-                                x[i][h] = -INFINITY;
-                                hide |= 1u << (2 * i + h);
+                        for (int c = 0; c < 4; ++c) {
+                            const int t = t0 + 8 * c + g;
+                            if (!(have >> (c >> 1) & 1) || t > row_pos[i] || (a.window > 0 && t <= row_pos[i] - a.window)) {
+                                x[i][c] = -INFINITY;
+                                hide |= 1u << (4 * i + c);
                             }
                         }
                 }
-                // The reference point m of a row's exponentials moves only when a
-                // score lies more than 2 above it: p stays below 4, and with a
+                // Scores are in units of 1 / rowf, rowf > 0.  The reference point m of
+                // a row's exponentials moves only when a score lies more than 2
+                // (as a power of two) above it: p stays below 4, and with a
                 // scale of at most 8736 p s stays a float16.
                 bool above = false;
 #pragma unroll
-                for (int i = 0; i < kR; ++i) above |= fmaxf(x[i][0], x[i][1]) > m[i] + 2.0f;
+                for (int i = 0; i < kR; ++i)
+                    above |= fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])) > limit[i];
                 if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                     for (int i = 0; i < kR; ++i) {
-                        float top = fmaxf(x[i][0], x[i][1]);
+                        float top = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
 #pragma unroll
                         for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                        const float keep = top > m[i] ? exp2_approx(m[i] - top) : 1.0f;
+                        const float keep = top > m[i] ? exp2_approx((m[i] - top) * rowf[i]) : 1.0f;
                         m[i] = fmaxf(m[i], top);
+                        limit[i] = m[i] + room[i];
+                        off[i] = m[i] == -INFINITY ? 0.0f : m[i] * rowf[i];
                         l[i] *= keep;
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
@@ -674,20 +716,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                 }
 #pragma unroll
                 for (int i = 0; i < kR; ++i) {
-                    const float off = m[i] == -INFINITY ? 0.0f : m[i];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        x[i][h] = exp2_approx(x[i][h] - off);
-                        l[i] += x[i][h];
-                    }
+                    for (int c = 0; c < 4; ++c) x[i][c] = exp2_approx(fmaf(x[i][c], rowf[i], -off[i]));
+                    l[i] += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
                 }
-                // The second product's B: row g, tokens 2 j + 8 h, + 1.
-                uint32_t pb[NT][G][2];
+                // The second product's B: row g, tokens 16 k + 8 h + 2 j, + 1.
+                uint32_t pb[2][NT][G][2];
                 auto weigh = [&](auto at_edge) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int c = 0; c < 4; ++c) {
                         uint32_t vp[G];
-                        const uint32_t at = st + 16 * D + 64 * G + (g + 8 * h) * G * 4;
+                        const uint32_t at = st0 + (c >> 1) * kGran + 16 * D + 64 * G + (g + 8 * (c & 1)) * G * 4;
                         if constexpr (G == 2) {
                             const uint2 v = lds64(at);
                             vp[0] = v.x, vp[1] = v.y;
@@ -700,13 +739,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                             float v[kR];
 #pragma unroll
                             for (int i = 0; i < kR; ++i) {
-                                v[i] = x[i][h] * p.x;
+                                v[i] = x[i][c] * p.x;
                                 if constexpr (at_edge) {   // a hidden token's params may be anything
-                                    const bool hidden = hide >> (2 * i + h) & 1;
+                                    const bool hidden = hide >> (4 * i + c) & 1;
                                     v[i] = hidden ? 0.0f : v[i];
-                                    w0[i][q] += hidden ? 0.0f : x[i][h] * p.y;
+                                    w0[i][q] += hidden ? 0.0f : x[i][c] * p.y;
                                 } else {
-                                    w0[i][q] = fmaf(x[i][h], p.y, w0[i][q]);
+                                    w0[i][q] = fmaf(x[i][c], p.y, w0[i][q]);
                                 }
                             }
 #pragma unroll
@@ -718,7 +757,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                                 } else {
                                     b = half2_bits(v[2 * n], v[2 * n + 1]);
                                 }
-                                pb[n][q][h] = transpose8x8(b);
+                                pb[c >> 1][n][q][c & 1] = transpose8x8(b);
                             }
                         }
                     }
@@ -726,29 +765,33 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                 if (edge) weigh(std::true_type{});
                 else weigh(std::false_type{});
                 // Values: lane's tokens 2 j, 2 j + 1 of each half, dims 64 q + 8 g + nibble.
-                uint32_t vw[2][2][G];   // [half][token][group]
-                if constexpr (G == 2) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint4 v = lds128(st + 8 * D + h * 512 + lane * 16);
-                        vw[h][0][0] = v.x, vw[h][0][1] = v.y, vw[h][1][0] = v.z, vw[h][1][1] = v.w;
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t st = st0 + k * kGran + 8 * D + lane * 16;
+                    uint32_t vw[2][2][G];   // [half][token][group]
+                    if constexpr (G == 2) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint4 v = lds128(st + h * 512);
+                            vw[h][0][0] = v.x, vw[h][0][1] = v.y, vw[h][1][0] = v.z, vw[h][1][1] = v.w;
+                        }
+                    } else {
+                        const uint4 v = lds128(st);
+                        vw[0][0][0] = v.x, vw[0][1][0] = v.y, vw[1][0][0] = v.z, vw[1][1][0] = v.w;
                     }
-                } else {
-                    const uint4 v = lds128(st + 8 * D + lane * 16);
-                    vw[0][0][0] = v.x, vw[0][1][0] = v.y, vw[1][0][0] = v.z, vw[1][1][0] = v.w;
+#pragma unroll
+                    for (int q = 0; q < G; ++q)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {   // byte i: nibbles 2 i (rows g) and 2 i + 1 (rows g + 8)
+                            const uint32_t sel = 0x0400 + 0x0101 * i;
+                            const uint32_t b0 = __byte_perm(vw[0][0][q], vw[0][1][q], sel);
+                            const uint32_t b1 = __byte_perm(vw[1][0][q], vw[1][1][q], sel);
+                            const uint32_t f[4] = {codes<kNormal>(b0, kEven), codes<kNormal>(b0, kOdd),
+                                                   codes<kNormal>(b1, kEven), codes<kNormal>(b1, kOdd)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(o[n][q][i], f, pb[k][n][q][0], pb[k][n][q][1]);
+                        }
                 }
-#pragma unroll
-                for (int q = 0; q < G; ++q)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {   // nibbles 2 i (rows g) and 2 i + 1 (rows g + 8)
-                        const uint32_t sel = i >> 1 ? 0x7632 : 0x5410;
-                        const uint32_t b0 = __byte_perm(vw[0][0][q], vw[0][1][q], sel) >> (8 * (i & 1));
-                        const uint32_t b1 = __byte_perm(vw[1][0][q], vw[1][1][q], sel) >> (8 * (i & 1));
-                        const uint32_t f[4] = {codes<kNormal>(b0, kEven), codes<kNormal>(b0, kOdd),
-                                               codes<kNormal>(b1, kEven), codes<kNormal>(b1, kOdd)};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_f16(o[n][q][i], f, pb[n][q][0], pb[n][q][1]);
-                    }
             }
             __syncwarp();
             issue((stage + kAttendStages - 1) % kAttendStages);
@@ -783,7 +826,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
                 *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
             }
             if (g == 0) {
-                res[kRows * kPitch + 2 * row] = m[i];
+                res[kRows * kPitch + 2 * row] = m[i] == -INFINITY ? -INFINITY : off[i];
                 res[kRows * kPitch + 2 * row + 1] = l[i];
             }
         }
@@ -791,10 +834,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
 
         const bool whole = first == 0 && last == rq.n;
         float* part = a.part + (2 * (long long)blockIdx.x + (first == 0 ? 1 : 0)) * kRows * (D + 2);
-        constexpr int kWarpFloats = kAttendStages * kGran / 4;
+        constexpr int kWarpFloats = kAttendStages * kStage / 4;
         auto write = [&](int row, int d, float4 v, float mm, float ll) {
             const int rr = tile * kRows + row;
-            const long long at = (long long)(rq.q0 + rr / Gh) * a.H + head * Gh + rr % Gh;
+            const int tok = a.group.div(rr);
+            const long long at = (long long)(rq.q0 + tok) * a.H + head * Gh + rr - tok * Gh;
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;    // no key seen: 0; a NaN stays one
             T* op = static_cast<T*>(a.out) + at * D + d;
             T t[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
@@ -827,13 +871,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
             }
         }
         if (!whole) {
-            // The blocks that hold its granules.
-            const long long c0 = (item_u + kAttendItemCost) / chunk, c1 = (item_u + length - 1) / chunk;
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) is_last = atomicAdd(a.counter + c0, 1) == (int)(c1 - c0);
+            if (threadIdx.x == 0) {   // the blocks that hold its granules
+                join_from = (int)((item_u + kAttendItemCost) / chunk);
+                join_to = (int)((item_u + length - 1) / chunk);
+                is_last = atomicAdd(a.counter + join_from, 1) == join_to - join_from;
+            }
             __syncthreads();
             if (is_last) {
+                const long long c0 = join_from, c1 = join_to;
                 __threadfence();
                 if (threadIdx.x == 0) a.counter[c0] = 0;
                 // The item begins in block c0 (its second part) and covers the
@@ -867,6 +914,29 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? 4 : 2) attend_ker
 }  // namespace
 }  // namespace moe
 
+using namespace moe;
+
+namespace {
+
+template <class T, int D> cudaError_t attend_attributes_of() {
+    const int smem = kAttendWarps * kAttendStages * 2 * kv4_granule(D);
+    cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attend_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return e;
+}
+
+template <int D> cudaError_t attend_attributes_dim() {
+    cudaError_t e = attend_attributes_of<float, D>();
+    if (e == cudaSuccess) e = attend_attributes_of<__nv_bfloat16, D>();
+    if (e == cudaSuccess) e = attend_attributes_of<__half, D>();
+    return e;
+}
+
+cudaError_t attend_attributes(int D) { return D == 64 ? attend_attributes_dim<64>() : attend_attributes_dim<128>(); }
+
+}  // namespace
+
 struct MoeKv4 {
     MoeKv4Config cfg;
     int sms = 0;
@@ -874,8 +944,6 @@ struct MoeKv4 {
     int* counter = nullptr;
     size_t bytes = 0;
 };
-
-using namespace moe;
 
 extern "C" {
 
@@ -900,6 +968,8 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
             return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_create: head_dim must be 64 or 128");
         if (cfg->block_tokens < 16 || cfg->block_tokens > 1024 || cfg->block_tokens % 16)
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: block_tokens must be a multiple of 16, 16..1024");
+        if ((long long)cfg->num_blocks * cfg->num_kv_heads * (cfg->block_tokens / 16) >= 0xffffffffll)
+            return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_create: a cache of 2^32 granules or more");
         if (cfg->num_blocks < 1 || cfg->table_width < 1 ||
             (long long)cfg->table_width * cfg->block_tokens > (1 << 30))
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: need num_blocks >= 1, table_width >= 1 and "
@@ -916,6 +986,7 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (2 * cfg->max_requests + 1) * (int)sizeof(int));
+        if (e == cudaSuccess) e = attend_attributes(cfg->head_dim);
         if (e != cudaSuccess) return launch_status(e, "moe_kv4_create");
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_create: cannot select the device");
         if (major != 10)
@@ -1000,7 +1071,7 @@ template <class T> cudaError_t append_dim(const AppendArgs& a, int D, bool vec, 
 
 template <class T, int D> cudaError_t attend_tiles(const AttendArgs& a, int sms, cudaStream_t s) {
     const dim3 block(kAttendWarps * 32);
-    const size_t smem = (size_t)kAttendWarps * kAttendStages * kv4_granule(D);
+    const size_t smem = (size_t)kAttendWarps * kAttendStages * 2 * kv4_granule(D);
     // Columns that a request's queries of one key/value head need on average.
     const long long columns = (long long)(a.H / a.Hkv) * ((a.tokens + a.R - 1) / a.R) * (sizeof(T) == 4 ? 2 : 1);
     return columns <= 8 ? launch(attend_kernel<T, D, 1>, sms * kAttendCtasPerSm, block, smem, s, false, a)
@@ -1075,7 +1146,8 @@ int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_attention_device: cannot select the device");
         AttendArgs a{static_cast<const uint8_t*>(cache), q, q_token_stride, q_head_stride, block_table, kv_len,
                      q_offset, out, lse, h->part, h->counter, tokens, num_heads, c.num_kv_heads, R, c.table_width, c.block_tokens,
-                     c.num_blocks, (long long)window >= (long long)c.table_width * c.block_tokens ? 0 : window, scale, false};
+                     c.num_blocks, (long long)window >= (long long)c.table_width * c.block_tokens ? 0 : window, scale, false,
+                     FastDiv(num_heads / c.num_kv_heads), FastDiv(c.block_tokens / 16)};
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         const int64_t es = (int64_t)dtype_bytes(dtype);
         a.vec = aligned16(q) && q_token_stride * es % 16 == 0 && q_head_stride * es % 16 == 0;
