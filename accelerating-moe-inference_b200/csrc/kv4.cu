@@ -293,6 +293,7 @@ struct AttendArgs {
     float* lse;
     float* part;      // [2 * grid][rows of a tile][D + 2]: unnormalised outputs, then m and l
     int* counter;     // [grid], zero between launches
+    volatile int* error;   // the handle's, in host memory
     int tokens, H, Hkv, R, W, bs, nb, window;
     float scale;
     bool vec;         // q rows can be read 16 bytes at a time
@@ -303,8 +304,8 @@ struct AttendArgs {
 constexpr int kAttendWarps = 4;
 constexpr int kAttendStages = 3;      // granule pairs in flight per warp
 constexpr int kAttendCtasPerSm = 3;
-constexpr int kAttendItemCost = 16;   // what an item costs beside its granules, in granules (measured: 17)
-constexpr int kAttendMinUnits = 24;
+constexpr int kAttendItemCost = 24;   // what an item costs beside its granules, in granules (measured: 25)
+constexpr int kAttendMinUnits = 12;
 constexpr int kAttendWhole = 8;       // items of up to so many granules are not cut: joining costs more
 
 // What one request asks for: its queries [q0, q0 + nq), cut length, the
@@ -317,9 +318,9 @@ struct Request {
 
 template <int kRows> __device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
     Request q;
-    q.q0 = min(max(a.q_offset[r], 0), a.tokens);
-    q.nq = min(max(a.q_offset[r + 1], q.q0), a.tokens) - q.q0;
-    q.len = (int)min((long long)max(a.kv_len[r], 0), (long long)a.W * a.bs);
+    q.q0 = min(max(__ldg(a.q_offset + r), 0), a.tokens);
+    q.nq = min(max(__ldg(a.q_offset + r + 1), q.q0), a.tokens) - q.q0;
+    q.len = (int)min((long long)max(__ldg(a.kv_len + r), 0), (long long)a.W * a.bs);
     q.lo = a.window > 0 ? max(0, q.len - q.nq - a.window + 1) >> 4 : 0;
     q.n = max(1, (int)(((long long)q.len + 15) >> 4) - q.lo);
     const int rows_per_head = q.nq * (a.H / a.Hkv);
@@ -345,6 +346,54 @@ template <bool kNormal> __device__ __forceinline__ uint32_t codes(uint32_t word,
     return v;
 }
 
+// Where a block stands in its units: the next item is `item` of request r, of
+// which `skip` units lie in earlier blocks; `left` units are still the block's.
+struct Walk {
+    int r, item, skip;
+    long long left;
+};
+
+// The block's next part of an item: granules [ga, gb) of key/value head `head`
+// for one tile of query rows.
+struct Segment {
+    int r, q0, head, tile, rows;
+    int base_pos, pos_lo, pos_hi;    // position of the request's query 0, of the tile's first and last row
+    int ga, gb;
+    int first, last, n;              // the item's granules that are the block's, of n
+    long long before;                // units of the block's before the item's first (may be negative)
+};
+
+template <int kRows> __device__ __forceinline__ bool next_segment(const AttendArgs& a, long long share, Walk& w, Segment& g) {
+    if (w.left <= 0) return false;
+    Request rq = request_of<kRows>(a, w.r);
+    while (w.item == rq.items) {         // units are left, so there is a next request
+        rq = request_of<kRows>(a, ++w.r);
+        w.item = 0;
+    }
+    const int length = rq.n + kAttendItemCost;
+    const long long count = rq.n <= kAttendWhole ? length : min((long long)(length - w.skip), w.left);
+    g.first = max(0, w.skip - kAttendItemCost);
+    g.last = (int)max(0ll, w.skip + count - kAttendItemCost);
+    g.n = rq.n;
+    g.before = share - w.left - w.skip;
+    const int Gh = a.group.d;
+    g.r = w.r;
+    g.q0 = rq.q0;
+    g.head = rq.tiles == 1 ? w.item : w.item / rq.tiles;
+    g.tile = w.item - g.head * rq.tiles;
+    g.rows = min(kRows, rq.nq * Gh - g.tile * kRows);
+    g.base_pos = rq.len - rq.nq;
+    g.pos_lo = g.base_pos + a.group.div(g.tile * kRows);
+    g.pos_hi = g.base_pos + a.group.div(g.tile * kRows + g.rows - 1);
+    g.ga = rq.lo + g.first;
+    g.gb = min(rq.lo + g.last, (g.pos_hi >> 4) + 1);       // pos_hi < 0: none
+    if (a.window > 0) g.ga = max(g.ga, max(0, g.pos_lo - a.window + 1) >> 4);
+    ++w.item;
+    w.skip = 0;
+    w.left -= count;
+    return g.last > 0;                   // else its granules all lie in later blocks, and the block is done
+}
+
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -361,9 +410,10 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // merges them in order of their place, so the result does not depend on the
 // order of arrival.
 //
-// A warp takes every fourth pair of granules of its block's run and keeps three of them
-// in flight by asynchronous copies into its own ring; no warp waits for
-// another before the run ends.
+// A warp takes every fourth pair of granules of its block's items and keeps
+// three pairs in flight by bulk copies into its own ring.  The copies
+// run through the block's items without regard to where one ends, so the next
+// item's granules are on their way while this one's rows are joined.
 //
 // Products: m16n8k16 with the cache as A (16 tokens, then 16 dims of the
 // transposed values) and the query rows as the 8 columns of B, so that few
@@ -395,16 +445,19 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     constexpr float kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     constexpr int kStage = 2 * kGran;
-    static_assert((kRows * kPitch + 2 * kRows) * 4 <= kAttendStages * kStage, "a warp's result fits its ring");
+    constexpr int kWarpFloats = kRows * kPitch + 2 * kRows;   // a warp's result
     extern __shared__ __align__(16) uint8_t attend_smem[];
     __shared__ long long scan_buf[33];
     __shared__ long long start_unit;
     __shared__ int start_r, is_last, join_from, join_to;
+    __shared__ Walk ahead_walk[kAttendWarps];
+    __shared__ uint64_t copies_done[kAttendWarps][kAttendStages];
+    __shared__ int2 ahead_run[kAttendWarps], ahead_where[kAttendWarps];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
     const int Gh = a.H / a.Hkv;
     uint8_t* ring = attend_smem + warp * kAttendStages * kStage;
-    const uint32_t ring_u = smem_u32(ring);
+    float* results = reinterpret_cast<float*>(attend_smem + kAttendWarps * kAttendStages * kStage);
 
     // The block's share of the units, and the request its first one lies in.
     const int per = (a.R + kThreads - 1) / kThreads;
@@ -427,88 +480,104 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
         }
     }
     __syncthreads();
-    int r = start_r;
-    Request rq = request_of<kRows>(a, r);
-    int item = (int)(start_unit / (rq.n + kAttendItemCost));
-    int skip = (int)(start_unit % (rq.n + kAttendItemCost));   // units of it that lie in earlier blocks
-    long long left = min(total - u0, chunk);
-    if (skip > 0 && rq.n <= kAttendWhole) {   // the block with its first unit has all of it
-        left -= rq.n + kAttendItemCost - skip;
-        ++item;
-        skip = 0;
-    }
-    const int page_grans = a.bs >> 4;                       // granules of a head in a page
-    const unsigned page_step = (unsigned)a.Hkv * page_grans;   // the granules of a cache are below 2^32 - 1
-
-    while (left > 0) {
-        if (item == rq.items) {
-            rq = request_of<kRows>(a, ++r);   // units are left, so there is one
-            item = 0;
-            continue;
+    Walk walk{start_r, 0, 0, min(total - u0, chunk)};
+    {
+        const Request rq = request_of<kRows>(a, start_r);
+        walk.item = (int)(start_unit / (rq.n + kAttendItemCost));
+        walk.skip = (int)(start_unit % (rq.n + kAttendItemCost));
+        if (walk.skip > 0 && rq.n <= kAttendWhole) {   // the block with its first unit has all of it
+            walk.left -= rq.n + kAttendItemCost - walk.skip;
+            ++walk.item;
+            walk.skip = 0;
         }
-        const int length = rq.n + kAttendItemCost;
-        const int count = rq.n <= kAttendWhole ? length : (int)min((long long)(length - skip), left);
-        const int first = max(0, skip - kAttendItemCost), last = max(0, skip + count - kAttendItemCost);
-        const long long item_u = u0 + min(total - u0, chunk) - left - skip;   // its first unit
-        const int head = rq.tiles == 1 ? item : item / rq.tiles, tile = item - head * rq.tiles;
-        ++item;
-        skip = 0;
-        left -= count;
-        if (last == 0) break;                 // its granules all lie in later blocks
-        const int rows = min(kRows, rq.nq * Gh - tile * kRows);
-        // Positions of the tile's first and last row, and the granules they see.
-        const int base_pos = rq.len - rq.nq;
-        const int pos_lo = base_pos + a.group.div(tile * kRows);
-        const int pos_hi = base_pos + a.group.div(tile * kRows + rows - 1);
-        int ga = rq.lo + first, gb = rq.lo + last;
-        if (a.window > 0) ga = max(ga, max(0, pos_lo - a.window + 1) >> 4);
-        gb = min(gb, (pos_hi >> 4) + 1);       // pos_hi < 0: none
+    }
+    const long long share = min(total - u0, chunk);
+    const int page_grans = a.bs >> 4;                          // granules of a head in a page
 
-        // Where the warp's granules lie, 16 pairs at a time: lane i holds the
-        // place in the cache of the i-th one, kNone without one or where its
-        // page is outside the pool; `later` the next 32's, loaded ahead.
-        constexpr unsigned kNone = 0xffffffffu;
-        const int* table = a.table + (size_t)r * a.W;
-        const uint8_t* head_base = a.cache + (long long)head * page_grans * kGran + lane * 16;
-        int ahead = ga + 2 * warp + (lane >> 1) * (2 * kAttendWarps) + (lane & 1);
-        auto locate = [&]() {
-            unsigned at = kNone;
-            if (ahead < gb) {
-                const int col = a.page.div(ahead), page = table[col];
-                if (page >= 0 && page < a.nb) at = (unsigned)page * page_step + (unsigned)(ahead - col * page_grans);
+    // Where the warp's granules lie, up to 16 pairs of one item at a time:
+    // lane i holds the place in the cache of the i-th one, kNone without one
+    // or where its page is outside the pool; `later` the batch after, loaded
+    // ahead.
+    constexpr unsigned kNone = 0xffffffffu;
+    Walk& ahead = ahead_walk[warp];
+    int2& run = ahead_run[warp];          // the granules of the item that are still to be placed
+    int2& where = ahead_where[warp];      // its request and head
+    if (lane == 0) {
+        ahead = walk;
+        run = make_int2(0, 0);
+    }
+    __syncwarp();
+    auto locate = [&](int& pairs) {
+        int2 left = run, rh = where;
+        while (left.x >= left.y) {
+            Walk w = ahead;
+            Segment sg;
+            if (!next_segment<kRows>(a, share, w, sg)) {
+                pairs = 0;
+                return kNone;
             }
-            ahead += 32 * kAttendWarps;
-            return at;
-        };
-        unsigned here = locate(), later = locate();
-        int pair = 0;
-        unsigned valid = 0;    // two bits per stage: there is such a granule
-        auto issue = [&](int stage) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const unsigned at = __shfl_sync(0xffffffffu, here, 2 * pair + k);
-                const unsigned bit = 1u << (2 * stage + k);
-                valid &= ~bit;
-                if (at != kNone) {
-                    valid |= bit;
-                    const uint8_t* src = head_base + (unsigned long long)at * kGran;
-                    const uint32_t dst = ring_u + stage * kStage + k * kGran + lane * 16;
-#pragma unroll
-                    for (int c = 0; c < kGran / 512; ++c) copy16_async(dst + c * 512, src + c * 512);
-                    if (kGran % 512 && lane < kGran % 512 / 16)
-                        copy16_async(dst + kGran / 512 * 512, src + kGran / 512 * 512);
-                }
+            left = make_int2(sg.ga + 2 * warp, sg.gb);
+            rh = make_int2(sg.r, sg.head);
+            __syncwarp();
+            if (lane == 0) {
+                ahead = w;
+                where = rh;
             }
-            copy_commit();
-            if (++pair == 16) {
-                pair = 0;
-                here = later;
-                later = locate();
-            }
-        };
+            __syncwarp();
+        }
+        unsigned at = kNone;
+        const int gi = left.x + (lane >> 1) * (2 * kAttendWarps) + (lane & 1);
+        if (gi < left.y) {
+            const int col = a.page.div(gi), page = __ldg(a.table + (size_t)rh.x * a.W + col);
+            if (page >= 0 && page < a.nb)
+                at = ((unsigned)page * a.Hkv + rh.y) * page_grans + (unsigned)(gi - col * page_grans);
+        }
+        pairs = min(16, (left.y - left.x + 2 * kAttendWarps - 1) / (2 * kAttendWarps));
+        __syncwarp();
+        if (lane == 0) run = make_int2(left.x + 32 * kAttendWarps, left.y);
+        __syncwarp();
+        return at;
+    };
+    int here_pairs, later_pairs, pair = 0;
+    unsigned here = locate(here_pairs), later = locate(later_pairs);
+    unsigned valid = 0;    // two bits per stage: there is such a granule
+    uint64_t* full = copies_done[warp];   // per stage: its copies have arrived
+    unsigned phases = 0;                  // the parity each stage's next wait is for
+    bool dead = false;                    // a wait ran out: no more copies
+    if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < kAttendStages - 1; ++s) issue(s);
+        for (int i = 0; i < kAttendStages; ++i) mbar_init(full + i, 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    auto issue = [&](int stage) {
+        if (pair == here_pairs) {
+            pair = 0;
+            here = later;
+            here_pairs = later_pairs;
+            if (here_pairs) later = locate(later_pairs);
+        }
+        valid &= ~(3u << (2 * stage));
+        if (here_pairs && !dead) {
+            const unsigned at0 = __shfl_sync(0xffffffffu, here, 2 * pair), at1 = __shfl_sync(0xffffffffu, here, 2 * pair + 1);
+            const unsigned have = (at0 != kNone ? 1u : 0u) | (at1 != kNone ? 2u : 0u);
+            valid |= have << (2 * stage);
+            if (have && lane == 0) {
+                uint8_t* dst = ring + stage * kStage;
+                mbar_arrive_expect_tx(full + stage, have == 3 ? kStage : kGran);
+                if (have & 1) bulk_load(dst, a.cache + (unsigned long long)at0 * kGran, kGran, full + stage);
+                if (have & 2) bulk_load(dst + kGran, a.cache + (unsigned long long)at1 * kGran, kGran, full + stage);
+            }
+            ++pair;
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kAttendStages - 1; ++s) issue(s);
 
+    int stage = 0;
+    Segment sg;
+    while (next_segment<kRows>(a, share, walk, sg)) {
+        const int rows = sg.rows, tile = sg.tile, head = sg.head;
         // The query fragments: rows scaled by a power of two to below 2^11,
         // dims of even nibbles another 16 up to match their codes' 2^-24.
         uint32_t qb[NT][D / 16][2];
@@ -521,7 +590,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             float x[2 * G][8];
             float mx = 0.0f;
             const int tok = a.group.div(row);
-            const T* qp = static_cast<const T*>(a.q) + (on ? (rq.q0 + tok) * a.q_token_stride +
+            const T* qp = static_cast<const T*>(a.q) + (on ? (sg.q0 + tok) * a.q_token_stride +
                                                               (head * Gh + row - tok * Gh) * a.q_head_stride : 0);
 #pragma unroll
             for (int w = 0; w < 2 * G; ++w) {
@@ -575,7 +644,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 rowf[n * kE + i] = __shfl_sync(0xffffffffu, f, src);
 #pragma unroll
                 for (int q = 0; q < G; ++q) qs[n * kE + i][q] = __shfl_sync(0xffffffffu, sum[q], src);
-                row_pos[n * kE + i] = base_pos + a.group.div(tile * kRows + (n * 8 + 2 * j) / kPlanes + i);
+                row_pos[n * kE + i] = sg.base_pos + a.group.div(tile * kRows + (n * 8 + 2 * j) / kPlanes + i);
             }
         }
 
@@ -598,27 +667,29 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                     for (int c = 0; c < 4; ++c) o[n][q][i][c] = 0.0f;
 
-        int stage = 0;
-        for (int gi = ga + 2 * warp; gi < gb; gi += 2 * kAttendWarps) {
-            copy_wait<kAttendStages - 2>();
-            __syncwarp();
-            const uint32_t st0 = ring_u + stage * kStage;
+        for (int gi = sg.ga + 2 * warp; gi < sg.gb; gi += 2 * kAttendWarps) {
+            const uint8_t* st0 = ring + stage * kStage;
             const unsigned have = valid >> (2 * stage) & 3;
             if (have) {
+                if (__any_sync(0xffffffffu, !mbar_wait(full + stage, phases >> stage & 1, nullptr, 0))) {
+                    dead = true;
+                    if (lane == 0) *a.error = kDevErrTimeoutProducer;
+                }
+                phases ^= 1u << stage;
                 // Scores x[row][2 k + h] of the lane's rows and tokens 16 k + g + 8 h.
                 float x[kR][4];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const uint32_t st = st0 + k * kGran;
+                    const uint8_t* st = st0 + k * kGran;
                     uint32_t kw[2][2 * G];
                     float acc[NT][G][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if constexpr (G == 2) {
-                            const uint4 v = lds128(st + h * 512 + lane * 16);
+                            const uint4 v = *reinterpret_cast<const uint4*>(st + h * 512 + lane * 16);
                             kw[h][0] = v.x, kw[h][1] = v.y, kw[h][2] = v.z, kw[h][3] = v.w;
                         } else {
-                            const uint2 v = lds64(st + h * 256 + lane * 8);
+                            const uint2 v = *reinterpret_cast<const uint2*>(st + h * 256 + lane * 8);
                             kw[h][0] = v.x, kw[h][1] = v.y;
                         }
                     }
@@ -641,12 +712,12 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t kp[G];
-                        const uint32_t at = st + 16 * D + (g + 8 * h) * G * 4;
+                        const uint8_t* at = st + 16 * D + (g + 8 * h) * G * 4;
                         if constexpr (G == 2) {
-                            const uint2 v = lds64(at);
+                            const uint2 v = *reinterpret_cast<const uint2*>(at);
                             kp[0] = v.x, kp[1] = v.y;
                         } else {
-                            kp[0] = lds32(at);
+                            kp[0] = *reinterpret_cast<const uint32_t*>(at);
                         }
                         float s[kR];
 #pragma unroll
@@ -665,7 +736,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                     }
                 }
                 const int t0 = gi << 4;
-                const bool edge = have != 3 || t0 + 31 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
+                const bool edge = have != 3 || t0 + 31 > sg.pos_lo || (a.window > 0 && t0 <= sg.pos_hi - a.window);
                 unsigned hide = 0;
                 if (edge) {
 #pragma unroll
@@ -726,12 +797,12 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t vp[G];
-                        const uint32_t at = st0 + (c >> 1) * kGran + 16 * D + 64 * G + (g + 8 * (c & 1)) * G * 4;
+                        const uint8_t* at = st0 + (c >> 1) * kGran + 16 * D + 64 * G + (g + 8 * (c & 1)) * G * 4;
                         if constexpr (G == 2) {
-                            const uint2 v = lds64(at);
+                            const uint2 v = *reinterpret_cast<const uint2*>(at);
                             vp[0] = v.x, vp[1] = v.y;
                         } else {
-                            vp[0] = lds32(at);
+                            vp[0] = *reinterpret_cast<const uint32_t*>(at);
                         }
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
@@ -767,16 +838,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 // Values: lane's tokens 2 j, 2 j + 1 of each half, dims 64 q + 8 g + nibble.
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const uint32_t st = st0 + k * kGran + 8 * D + lane * 16;
+                    const uint8_t* st = st0 + k * kGran + 8 * D + lane * 16;
                     uint32_t vw[2][2][G];   // [half][token][group]
                     if constexpr (G == 2) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint4 v = lds128(st + h * 512);
+                            const uint4 v = *reinterpret_cast<const uint4*>(st + h * 512);
                             vw[h][0][0] = v.x, vw[h][0][1] = v.y, vw[h][1][0] = v.z, vw[h][1][1] = v.w;
                         }
                     } else {
-                        const uint4 v = lds128(st);
+                        const uint4 v = *reinterpret_cast<const uint4*>(st);
                         vw[0][0][0] = v.x, vw[0][1][0] = v.y, vw[1][0][0] = v.z, vw[1][1][0] = v.w;
                     }
 #pragma unroll
@@ -797,11 +868,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             issue((stage + kAttendStages - 1) % kAttendStages);
             stage = (stage + 1) % kAttendStages;
         }
-        copy_wait<0>();
-        __syncwarp();
-
-        // The warp's rows into its ring's place: output, then m and l.
-        float* res = reinterpret_cast<float*>(ring);
+        // The warp's rows: output, then m and l.
+        __syncthreads();   // the last item's are read
+        float* res = results + warp * kWarpFloats;
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
             const int row = (i / kE * 8 + 2 * j) / kPlanes + i % kE;
@@ -832,13 +901,12 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
         }
         __syncthreads();
 
-        const bool whole = first == 0 && last == rq.n;
-        float* part = a.part + (2 * (long long)blockIdx.x + (first == 0 ? 1 : 0)) * kRows * (D + 2);
-        constexpr int kWarpFloats = kAttendStages * kStage / 4;
+        const bool whole = sg.first == 0 && sg.last == sg.n;
+        float* part = a.part + (2 * (long long)blockIdx.x + (sg.first == 0 ? 1 : 0)) * kRows * (D + 2);
         auto write = [&](int row, int d, float4 v, float mm, float ll) {
             const int rr = tile * kRows + row;
             const int tok = a.group.div(rr);
-            const long long at = (long long)(rq.q0 + tok) * a.H + head * Gh + rr - tok * Gh;
+            const long long at = (long long)(sg.q0 + tok) * a.H + head * Gh + rr - tok * Gh;
             const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;    // no key seen: 0; a NaN stays one
             T* op = static_cast<T*>(a.out) + at * D + d;
             T t[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
@@ -849,7 +917,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
         };
         for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
-            const float* w = reinterpret_cast<const float*>(attend_smem);
+            const float* w = results;
             float mm = -INFINITY, ll = 0.0f;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
@@ -874,8 +942,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {   // the blocks that hold its granules
-                join_from = (int)((item_u + kAttendItemCost) / chunk);
-                join_to = (int)((item_u + length - 1) / chunk);
+                const long long item = u0 + sg.before + kAttendItemCost;
+                join_from = (int)(item / chunk);
+                join_to = (int)((item + sg.n - 1) / chunk);
                 is_last = atomicAdd(a.counter + join_from, 1) == join_to - join_from;
             }
             __syncthreads();
@@ -891,6 +960,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                     const int row = i / (D / 4), d = i % (D / 4) * 4;
                     float mm = -INFINITY, ll = 0.0f;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
                     for (long long c = c0; c <= c1; ++c) {
                         const float* p = p0 + (c - c0) * step - (c > c0 ? kRows * (D + 2) : 0) + row * (D + 2);
                         const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + D));
@@ -907,7 +977,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 }
             }
         }
-        __syncthreads();   // the rings and is_last are free again
     }
 }
 
@@ -918,11 +987,17 @@ using namespace moe;
 
 namespace {
 
+// The warps' rings, then their results.
+template <class T, int D, int NT> constexpr int attend_smem_bytes() {
+    return kAttendWarps * (kAttendStages * 2 * kv4_granule(D) + 8 * NT / (sizeof(T) == 4 ? 2 : 1) * (D + 4 + 2) * 4);
+}
+
 template <class T, int D> cudaError_t attend_attributes_of() {
-    const int smem = kAttendWarps * kAttendStages * 2 * kv4_granule(D);
-    cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         attend_smem_bytes<T, D, 1>());
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(attend_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = cudaFuncSetAttribute(attend_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 attend_smem_bytes<T, D, 2>());
     return e;
 }
 
@@ -942,6 +1017,7 @@ struct MoeKv4 {
     int sms = 0;
     float* part = nullptr;     // attention: partial rows of items that several blocks share
     int* counter = nullptr;
+    int* error = nullptr;      // pinned host memory: a kernel's wait ran out
     size_t bytes = 0;
 };
 
@@ -1001,6 +1077,8 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
         if (e == cudaSuccess) e = cudaMalloc(&h->counter, counter);
         if (e == cudaSuccess) e = cudaMemset(h->counter, 0, counter);
         if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        if (e == cudaSuccess) e = cudaHostAlloc(reinterpret_cast<void**>(&h->error), sizeof(int), cudaHostAllocMapped);
+        if (e == cudaSuccess) *h->error = 0;
         if (e != cudaSuccess) {
             cudaGetLastError();
             moe_kv4_destroy(h);
@@ -1018,6 +1096,7 @@ void moe_kv4_destroy(MoeKv4* h) {
     OnDevice on(h->cfg.device);
     cudaFree(h->part);
     cudaFree(h->counter);
+    cudaFreeHost(h->error);
     delete h;
 }
 
@@ -1071,11 +1150,11 @@ template <class T> cudaError_t append_dim(const AppendArgs& a, int D, bool vec, 
 
 template <class T, int D> cudaError_t attend_tiles(const AttendArgs& a, int sms, cudaStream_t s) {
     const dim3 block(kAttendWarps * 32);
-    const size_t smem = (size_t)kAttendWarps * kAttendStages * 2 * kv4_granule(D);
     // Columns that a request's queries of one key/value head need on average.
     const long long columns = (long long)(a.H / a.Hkv) * ((a.tokens + a.R - 1) / a.R) * (sizeof(T) == 4 ? 2 : 1);
-    return columns <= 8 ? launch(attend_kernel<T, D, 1>, sms * kAttendCtasPerSm, block, smem, s, false, a)
-                        : launch(attend_kernel<T, D, 2>, sms * 2, block, smem, s, false, a);
+    return columns <= 8
+               ? launch(attend_kernel<T, D, 1>, sms * kAttendCtasPerSm, block, attend_smem_bytes<T, D, 1>(), s, false, a)
+               : launch(attend_kernel<T, D, 2>, sms * 2, block, attend_smem_bytes<T, D, 2>(), s, false, a);
 }
 
 template <class T> cudaError_t attend_dim(const AttendArgs& a, int D, int sms, cudaStream_t s) {
@@ -1142,10 +1221,13 @@ int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_
         if (!aligned16(cache) || !aligned16(out) || !aligned_to(q, dtype_bytes(dtype)))
             return report_error(MOE_ERR_INVALID, "moe_kv4_attention_device: cache and out must be 16-byte aligned, q "
                                                  "to its elements");
+        if (*static_cast<volatile int*>(h->error))
+            return report_error(MOE_ERR_TIMEOUT, "moe_kv4_attention_device: a copy of an earlier call did not arrive "
+                                                 "in time; its results, and this handle, are not to be used");
         OnDevice on(c.device);
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_attention_device: cannot select the device");
         AttendArgs a{static_cast<const uint8_t*>(cache), q, q_token_stride, q_head_stride, block_table, kv_len,
-                     q_offset, out, lse, h->part, h->counter, tokens, num_heads, c.num_kv_heads, R, c.table_width, c.block_tokens,
+                     q_offset, out, lse, h->part, h->counter, h->error, tokens, num_heads, c.num_kv_heads, R, c.table_width, c.block_tokens,
                      c.num_blocks, (long long)window >= (long long)c.table_width * c.block_tokens ? 0 : window, scale, false,
                      FastDiv(num_heads / c.num_kv_heads), FastDiv(c.block_tokens / 16)};
         const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -610,7 +610,8 @@ int moe_kv4_append_device(MoeKv4* h, void* cache, const void* k, const void* v, 
  * table's width is cut to it; keys on a page outside the pool are not seen.
  * Scores, softmax and sums are in fp32; q and the probabilities enter the
  * products as float16 with 11 significant bits for 16-bit types and 22 for
- * fp32. */
+ * fp32.  The kernel's waits are bounded; once one has run out (its results are
+ * then undefined), every later call on the handle returns MOE_ERR_TIMEOUT. */
 int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_t dtype,
                              int32_t tokens, int32_t num_heads, int64_t q_token_stride,
                              int64_t q_head_stride, const int32_t* block_table,
