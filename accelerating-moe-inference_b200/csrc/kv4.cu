@@ -678,63 +678,66 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 phases ^= 1u << stage;
                 // Scores x[row][2 k + h] of the lane's rows and tokens 16 k + g + 8 h.
                 float x[kR][4];
+                float acc[2][NT][G][4];
+                uint32_t kw[2][2][2 * G];   // [granule][half][word]
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint8_t* st = st0 + k * kGran;
-                    uint32_t kw[2][2 * G];
-                    float acc[NT][G][4];
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        const uint8_t* at = st0 + k * kGran + h * 8 * (D / 2) + lane * (D / 8);
                         if constexpr (G == 2) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(st + h * 512 + lane * 16);
-                            kw[h][0] = v.x, kw[h][1] = v.y, kw[h][2] = v.z, kw[h][3] = v.w;
+                            const uint4 v = *reinterpret_cast<const uint4*>(at);
+                            kw[k][h][0] = v.x, kw[k][h][1] = v.y, kw[k][h][2] = v.z, kw[k][h][3] = v.w;
                         } else {
-                            const uint2 v = *reinterpret_cast<const uint2*>(st + h * 256 + lane * 8);
-                            kw[h][0] = v.x, kw[h][1] = v.y;
+                            const uint2 v = *reinterpret_cast<const uint2*>(at);
+                            kw[k][h][0] = v.x, kw[k][h][1] = v.y;
                         }
                     }
+                // The sums of the two granules and groups in turn, so that a
+                // product does not wait for the one before it.
 #pragma unroll
-                    for (int q = 0; q < G; ++q) {
+                for (int step = 0; step < 4; ++step)
 #pragma unroll
-                        for (int w = 2 * q; w < 2 * q + 2; ++w)
+                    for (int q = 0; q < G; ++q)
 #pragma unroll
-                            for (int half = 0; half < 2; ++half) {
-                                const uint32_t lo = kw[0][w] >> (8 * half), hi = kw[1][w] >> (8 * half);
-                                const uint32_t f[4] = {codes<kNormal>(lo, kEven), codes<kNormal>(hi, kEven),
-                                                       codes<kNormal>(lo, kOdd), codes<kNormal>(hi, kOdd)};
+                        for (int k = 0; k < 2; ++k) {
+                            const int w = 2 * q + (step >> 1), shift = 8 * (step & 1);
+                            const uint32_t lo = kw[k][0][w] >> shift, hi = kw[k][1][w] >> shift;
+                            const uint32_t f[4] = {codes<kNormal>(lo, kEven), codes<kNormal>(hi, kEven),
+                                                   codes<kNormal>(lo, kOdd), codes<kNormal>(hi, kOdd)};
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    if (w == 2 * q && half == 0) mma_f16_first(acc[n][q], f, qb[n][2 * w][0], qb[n][2 * w][1]);
-                                    else mma_f16(acc[n][q], f, qb[n][2 * w + half][0], qb[n][2 * w + half][1]);
-                                }
+                            for (int n = 0; n < NT; ++n) {
+                                const uint32_t(&b)[2] = qb[n][2 * w + (step & 1)];
+                                if (step == 0) mma_f16_first(acc[k][n][q], f, b[0], b[1]);
+                                else mma_f16(acc[k][n][q], f, b[0], b[1]);
                             }
-                    }
+                        }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t kp[G];
-                        const uint8_t* at = st + 16 * D + (g + 8 * h) * G * 4;
+                        const uint8_t* at = st0 + k * kGran + 16 * D + (g + 8 * h) * G * 4;
                         if constexpr (G == 2) {
                             const uint2 v = *reinterpret_cast<const uint2*>(at);
                             kp[0] = v.x, kp[1] = v.y;
                         } else {
                             kp[0] = *reinterpret_cast<const uint32_t*>(at);
                         }
-                        float s[kR];
 #pragma unroll
-                        for (int q = 0; q < G; ++q) {
-                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
+                        for (int i = 0; i < kR; ++i) {
+                            float s = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < kR; ++i) {
-                                const float (&t)[4] = acc[i / kE][q];
+                            for (int q = 0; q < G; ++q) {
+                                const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
+                                const float (&t)[4] = acc[k][i / kE][q];
                                 const float d = kPlanes == 2 ? fmaf(t[2 * h + 1], kLo, t[2 * h]) : t[2 * h + i % kE];
-                                s[i] = q == 0 ? p.y * qs[i][q] : fmaf(p.y, qs[i][q], s[i]);
-                                s[i] = fmaf(p.x, d, s[i]);
+                                s = q == 0 ? p.y * qs[i][q] : fmaf(p.y, qs[i][q], s);
+                                s = fmaf(p.x, d, s);
                             }
+                            x[i][2 * k + h] = s;
                         }
-#pragma unroll
-                        for (int i = 0; i < kR; ++i) x[i][2 * k + h] = s[i];
                     }
-                }
                 const int t0 = gi << 4;
                 const bool edge = have != 3 || t0 + 31 > sg.pos_lo || (a.window > 0 && t0 <= sg.pos_hi - a.window);
                 unsigned hide = 0;
