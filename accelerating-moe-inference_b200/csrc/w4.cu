@@ -4,59 +4,402 @@
 #include <new>
 
 #include "dtype.cuh"
+#include "mma.cuh"
 #include "moe_internal.h"
+#include "ptx.cuh"
 
 namespace moe {
 namespace {
 
-struct W4Args {
+constexpr int kMaxRows = 512;        // products of one call
+constexpr int kBlockK = 128;         // columns of a record
+constexpr int kWarps = 8;
+
+// The handle's own layout of the weights: records of 16 rows x 128 columns,
+// [matrix][tile of 16 rows][block of 128 columns].  Lane 4 g + j of a warp
+// owns, of rows g and g + 8, the columns 32 w + 8 j .. + 7 of each w < 4:
+//   codes   [row half][lane][4 w] 32-bit words, the lowest nibble first
+//   params  [8 g][row half][128 / group] (scale, zero) float16 pairs
+// so that a warp reads a record with whole 512-byte loads and each lane has
+// the operands of m16n8k16 products in its own registers.  A gated matrix has
+// tile 2 i from the gate rows and tile 2 i + 1 from the same up rows.  Rows
+// and columns of the padding have scale 0.
+__host__ __device__ constexpr int w4_record(int groups) { return 1024 + 64 * groups; }
+
+struct PackArgs {
     const uint8_t* codes;
     const __half* scales;
     const uint8_t* zeros;
-    const void* x;
-    const int* matrix;
-    void* y;
-    long long x_stride;
-    int rows, x_share, E, N, K, group, outputs;
+    uint8_t* out;
+    int rows, cols, group, tiles, blocks;
     bool gated;
 };
 
-template <class T> __device__ float row_dot(const W4Args& a, int e, int n, const T* x, int lane) {
-    const long long row = (long long)e * a.N + n;
-    const uint8_t* c = a.codes + row * (a.K / 2);
-    const int groups = (a.K + a.group - 1) / a.group;
-    float sum = 0.0f;
-    for (int k = lane * 8; k < a.K; k += 256) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(c + k / 2);
-        const long long g = row * groups + k / a.group;
-        const float z = a.zeros ? (float)a.zeros[g] : 8.0f, s = __half2float(a.scales[g]);
-        float part = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) part = fmaf((float)((w >> (4 * i)) & 15) - z, to_f32(x[k + i]), part);
-        sum = fmaf(s, part, sum);
+// One block per record of one matrix; thread = (half, lane, half word pair).
+__global__ void __launch_bounds__(256) w4_pack_kernel(PackArgs a) {
+    const int block = blockIdx.x % a.blocks, tile = blockIdx.x / a.blocks, per = kBlockK / a.group;
+    const long long matrix = blockIdx.y;
+    uint8_t* rec = a.out + ((matrix * a.tiles + tile) * a.blocks + block) * w4_record(per);
+    const int half_rows = a.gated ? a.rows / 2 : a.rows;
+    auto row_of = [&](int r) {      // source row of the tile's row r, -1 for padding
+        const int at = (a.gated ? tile >> 1 : tile) * 16 + r;
+        return at < half_rows ? at + (a.gated && (tile & 1) ? half_rows : 0) : -1;
+    };
+    {
+        const int w = threadIdx.x & 3, lane = threadIdx.x >> 2 & 31, half = threadIdx.x >> 7;
+        const int row = row_of((lane >> 2) + 8 * half), k = block * kBlockK + 32 * w + 8 * (lane & 3);
+        uint32_t v = 0;
+        if (row >= 0 && k < a.cols)
+            v = *reinterpret_cast<const uint32_t*>(a.codes + (matrix * a.rows + row) * (a.cols / 2) + k / 2);
+        reinterpret_cast<uint32_t*>(rec)[threadIdx.x] = v;
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+    if (threadIdx.x < 16 * per) {
+        const int q = threadIdx.x % per, half = threadIdx.x / per & 1, g = threadIdx.x / per / 2;
+        const int row = row_of(g + 8 * half), k = block * kBlockK + q * a.group;
+        const int groups = (a.cols + a.group - 1) / a.group;
+        __half s = __float2half_rn(0.0f), z = s;
+        if (row >= 0 && k < a.cols) {
+            const long long at = (matrix * a.rows + row) * groups + k / a.group;
+            s = a.scales[at];
+            z = __float2half_rn(a.zeros ? (float)a.zeros[at] : 8.0f);
+        }
+        reinterpret_cast<__half2*>(rec + 1024)[threadIdx.x] = __halves2half2(s, z);
+    }
 }
 
-// One warp per output.
-template <class TX, class TY> __global__ void __launch_bounds__(256) matvec_kernel(W4Args a) {
-    const int lane = threadIdx.x & 31, n = blockIdx.x * 8 + (threadIdx.x >> 5), i = blockIdx.y;
-    if (n >= a.outputs) return;
-    const int e = a.matrix ? a.matrix[i] : 0;
-    float v = 0.0f;
-    if (e >= 0 && e < a.E) {
-        const TX* x = static_cast<const TX*>(a.x) + (i / a.x_share) * a.x_stride;
-        v = row_dot(a, e, n, x, lane);
-        if (a.gated) v = v / (1.0f + expf(-v)) * row_dot(a, e, n + a.outputs, x, lane);
+// ------------------------------------------------------------ activations
+// A row of activations as the products' operand: scaled by a power of two to
+// below 2^11, as one float16 plane (16-bit types: exact down to 2^-34 of the
+// row's largest) or two, hi and (x - hi) 2^11 (fp32: 22 bits).
+//   plane   [row][plane][block of 128][4 w][4 j] 16 bytes: the float16 pairs
+//           (i, i + 4), i < 4, of columns 32 w + 8 j .. + 7; with one plane
+//           those of even i times 16 to match their codes' 2^-24
+//   sums    [row][blocks * 128 / group] of the scaled values
+//   unit    [row] what a scaled sum is multiplied by
+struct Planes {
+    uint4* plane;
+    float* sums;
+    float* unit;
+};
+
+template <class T, int kPlanes>
+__global__ void __launch_bounds__(512) w4_planes_kernel(const T* x, long long stride, int cols, int blocks, int group, Planes out) {
+    __shared__ float best[16];
+    const int row = blockIdx.x;
+    const T* p = x + row * stride;
+    wait_predecessor_grid();
+    launch_dependents();
+    float mx = 0.0f;
+    for (int k = threadIdx.x; k < cols; k += 512) mx = fmaxf(mx, fabsf(to_f32(p[k])));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mx;
+    __syncthreads();
+    mx = best[threadIdx.x & 15];
+#pragma unroll
+    for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    // Exponent of the largest, kept where 2^(10 - e) is a normal number.
+    const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
+    const float up = __uint_as_float((264 - e) << 23);
+    if (threadIdx.x == 0) out.unit[row] = __uint_as_float((e - 10) << 23);
+    const int chunks = blocks * (kBlockK / 8), per = group / 8;
+    for (int c = threadIdx.x; c < chunks; c += 512) {    // chunks is a multiple of 16: whole groups of lanes
+        float v[8], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += v[i] = c * 8 < cols ? to_f32(p[c * 8 + i]) * up : 0.0f;
+        const unsigned live = __activemask();
+        for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
+        if (c % per == 0) out.sums[(long long)row * (chunks / per) + c / per] = sum;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = kPlanes == 2 || (i & 1) ? 1.0f : 16.0f;
+            const __half2 h = __floats2half2_rn(v[i] * f, v[i + 4] * f);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+            if constexpr (kPlanes == 2) {
+                const float2 b = __half22float2(h);
+                const __half2 l = __floats2half2_rn((v[i] * f - b.x) * 2048.0f, (v[i + 4] * f - b.y) * 2048.0f);
+                lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+            }
+        }
+        uint4* to = out.plane + (long long)row * kPlanes * chunks + c;
+        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (kPlanes == 2) to[chunks] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    if (lane == 0) static_cast<TY*>(a.y)[(long long)i * a.outputs + n] = from_f32<TY>(v);
+}
+
+// --------------------------------------------------------------- products
+struct MatvecArgs {
+    const uint8_t* records;
+    Planes x;
+    const int* matrix;      // [num_rows], or null
+    void* y;                // [num_rows][outputs]
+    int num_rows, x_share, E, tiles, blocks, outputs, dtype;
+    bool gated;
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ void store_as(void* y, long long at, float v, int dtype) {
+    if (dtype == MOE_DTYPE_F32) static_cast<float*>(y)[at] = v;
+    else if (dtype == MOE_DTYPE_BF16) static_cast<__nv_bfloat16*>(y)[at] = from_f32<__nv_bfloat16>(v);
+    else static_cast<__half*>(y)[at] = from_f32<__half>(v);
+}
+
+// y = W x for the rows of x that ask for one matrix; a block has MT tiles of 16
+// weight rows, its warps every eighth block of 128 columns.
+//
+// Bound by reading the weights, so a warp streams its records straight into
+// registers, kDepth of them ahead (the first ones before the activations'
+// kernel has ended), and no weight passes through shared memory.  Products:
+// m16n8k16 with the codes as A and up to 8 NT columns of activations (a row of
+// x, or one of its two planes) as B.  A 4-bit code in the low bits of a
+// float16 word is the subnormal c 2^-24 (c 2^-20 four bits higher): one AND
+// makes an operand of two codes.  With one plane the zero is taken off after
+// the group's sum, s (sum(c x) - z sum(x)); with two (fp32), where the sum's
+// last bits count, code and zero become the normal number (c - z) 2^-10 by one
+// fma.  The warps' sums are added in order through shared memory.
+template <int kPlanes, int MT, int NT, int kPer>
+__global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel(MatvecArgs a) {
+    constexpr int kCols = 8 * NT, kTokens = kCols / kPlanes;     // products per pass
+    constexpr int kV = kPlanes == 2 ? 2 : 4;                     // sums per lane, tile and column tile
+    constexpr int kDepth = 2;
+    constexpr int kRecord = w4_record(kPer);
+    constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
+    __shared__ float part[kWarps][MT * 16][kTokens + 1];
+    __shared__ short list[kMaxRows];
+    __shared__ int list_n;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    const int tile = blockIdx.x * MT;
+
+    // The products that ask for this block's matrix, in order.
+    int matrix = 0, n = a.num_rows;
+    if (a.matrix) {
+        matrix = blockIdx.y;
+        if (warp == 0) {
+            int count = 0;
+            for (int i = 0; i < a.num_rows; i += 32) {
+                const bool mine = i + lane < a.num_rows && __ldg(a.matrix + i + lane) == matrix;
+                const unsigned m = __ballot_sync(0xffffffffu, mine);
+                if (mine) list[count + __popc(m & ((1u << lane) - 1))] = (short)(i + lane);
+                count += __popc(m);
+            }
+            if (lane == 0) list_n = count;
+        }
+        __syncthreads();
+        n = list_n;
+        if (matrix == 0) {   // zeros for the products without a matrix
+            wait_predecessor_grid();
+            const int first = (a.gated ? tile / 2 : tile) * 16, rows = min(a.gated ? MT * 8 : MT * 16, a.outputs - first);
+            for (int i = warp; i < a.num_rows; i += kWarps) {
+                const int m = __ldg(a.matrix + i);
+                if (m >= 0 && m < a.E) continue;
+                for (int r = lane; r < rows; r += 32) store_as(a.y, (long long)i * a.outputs + first + r, 0.0f, a.dtype);
+            }
+        }
+        if (n == 0) return;
+    }
+    const uint8_t* base = a.records + ((long long)matrix * a.tiles + tile) * a.blocks * kRecord;
+    const long long tile_step = (long long)a.blocks * kRecord;
+
+    struct Raw {
+        uint4 code[MT][2];
+        uint32_t par[MT][2 * kPer];
+    };
+    Raw raw[kDepth];
+    auto fetch = [&](Raw& r, int kb) {
+        if (kb < a.blocks) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const uint8_t* rec = base + t * tile_step + (long long)kb * kRecord;
+                r.code[t][0] = load_stream(reinterpret_cast<const uint4*>(rec) + lane);
+                r.code[t][1] = load_stream(reinterpret_cast<const uint4*>(rec + 512) + lane);
+                const uint8_t* p = rec + 1024 + g * (8 * kPer);
+                if constexpr (kPer == 1) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                    r.par[t][0] = v.x, r.par[t][1] = v.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2 * kPer; i += 4) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+                        r.par[t][i] = v.x, r.par[t][i + 1] = v.y, r.par[t][i + 2] = v.z, r.par[t][i + 3] = v.w;
+                    }
+                }
+            }
+        }
+    };
+
+    for (int t0 = 0; t0 < n; t0 += kTokens) {
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) fetch(raw[d], warp + d * kWarps);
+        if (t0 == 0) {
+            wait_predecessor_grid();
+            launch_dependents();
+        }
+        // The lane's column of B, and the rows whose sums it holds.
+        const uint4* bx[NT];
+        const float* sx[NT][2 / kPlanes];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            auto x_row = [&](int token) {
+                const int i = min(t0 + token, n - 1);
+                return (a.matrix ? list[i] : i) / a.x_share;
+            };
+            const int col = c * 8 + g, token = col / kPlanes;
+            const long long per_row = (long long)a.blocks * 16;
+            bx[c] = t0 + token < n ? a.x.plane + (x_row(token) * kPlanes + col % kPlanes) * per_row + j : nullptr;
+#pragma unroll
+            for (int i = 0; i < 2 / kPlanes; ++i)
+                sx[c][i] = a.x.sums + (long long)x_row((c * 8 + 2 * j) / kPlanes + i) * a.blocks * kPer;
+        }
+        uint4 bw[kDepth][NT][4];
+        auto fetch_x = [&](uint4 (&b)[NT][4], int kb) {
+            if (kb < a.blocks) {
+#pragma unroll
+                for (int c = 0; c < NT; ++c)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        b[c][w] = bx[c] ? __ldg(bx[c] + kb * 16 + w * 4) : make_uint4(0, 0, 0, 0);
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) fetch_x(bw[d], warp + d * kWarps);
+
+        float y[MT][NT][kV];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int i = 0; i < kV; ++i) y[t][c][i] = 0.0f;
+
+        for (int kb0 = warp; kb0 < a.blocks; kb0 += kDepth * kWarps) {
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d) {
+                const int kb = kb0 + d * kWarps;
+                if (kb >= a.blocks) break;
+                float sums[NT][2][kPer];
+                if constexpr (kPlanes == 1) {
+#pragma unroll
+                    for (int c = 0; c < NT; ++c)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int q = 0; q < kPer; ++q) sums[c][i][q] = __ldg(sx[c][i] + kb * kPer + q);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const uint4 c0 = raw[d].code[t][0], c1 = raw[d].code[t][1];
+                    const uint32_t lo[4] = {c0.x, c0.y, c0.z, c0.w}, hi[4] = {c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) {
+                        float acc[NT][4];
+                        __half2 zero[2];
+                        if constexpr (kPlanes == 2) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                zero[h] = __hmul2(__high2half2(*reinterpret_cast<const __half2*>(&raw[d].par[t][h * kPer + q])),
+                                                  __float2half2_rn(-1.0f / 1024.0f));
+                        }
+                        auto operand = [&](uint32_t word, uint32_t mask, int h) -> uint32_t {
+                            uint32_t v = word & mask;
+                            if constexpr (kPlanes == 2) {
+                                const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v),
+                                                          __float2half2_rn(mask == kEven ? 16384.0f : 1024.0f), zero[h]);
+                                v = *reinterpret_cast<const uint32_t*>(&r);
+                            }
+                            return v;
+                        };
+#pragma unroll
+                        for (int w = q * (4 / kPer); w < (q + 1) * (4 / kPer); ++w)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const uint32_t l = lo[w] >> (8 * half), u = hi[w] >> (8 * half);
+                                const uint32_t f[4] = {operand(l, kEven, 0), operand(u, kEven, 1),
+                                                       operand(l, kOdd, 0), operand(u, kOdd, 1)};
+#pragma unroll
+                                for (int c = 0; c < NT; ++c) {
+                                    const uint4 b = bw[d][c][w];
+                                    const uint32_t b0 = half ? b.z : b.x, b1 = half ? b.w : b.y;
+                                    if (w == q * (4 / kPer) && half == 0) mma_f16_first(acc[c], f, b0, b1);
+                                    else mma_f16(acc[c], f, b0, b1);
+                                }
+                            }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&raw[d].par[t][h * kPer + q]));
+#pragma unroll
+                            for (int c = 0; c < NT; ++c) {
+                                if constexpr (kPlanes == 2) {
+                                    y[t][c][h] = fmaf(p.x, fmaf(acc[c][2 * h + 1], 1.0f / 2048.0f, acc[c][2 * h]), y[t][c][h]);
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < 2; ++i) {
+                                        // acc is in units of 2^-20, the sums in ones.
+                                        const float v = fmaf(acc[c][2 * h + i], 1048576.0f, -p.y * sums[c][i][q]);
+                                        y[t][c][2 * h + i] = fmaf(p.x, v, y[t][c][2 * h + i]);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+                fetch(raw[d], kb + kDepth * kWarps);
+                fetch_x(bw[d], kb + kDepth * kWarps);
+            }
+        }
+        __syncthreads();   // the last pass's sums are read
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (kPlanes == 2) {
+                        part[warp][t * 16 + 8 * h + g][c * 4 + j] = y[t][c][h];
+                    } else {
+                        part[warp][t * 16 + 8 * h + g][c * 8 + 2 * j] = y[t][c][2 * h];
+                        part[warp][t * 16 + 8 * h + g][c * 8 + 2 * j + 1] = y[t][c][2 * h + 1];
+                    }
+                }
+        __syncthreads();
+        const int now = min(kTokens, n - t0);
+        const int out_rows = a.gated ? MT * 8 : MT * 16;
+        for (int i = threadIdx.x; i < out_rows * now; i += kWarps * 32) {
+            const int r = i % out_rows, token = i / out_rows;
+            const int slot = a.matrix ? list[t0 + token] : t0 + token;
+            const float unit = __ldg(a.x.unit + slot / a.x_share) * (kPlanes == 2 ? 1024.0f : 1.0f);
+            auto total = [&](int row) {
+                float v = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) v += part[k][row][token];
+                return v * unit;
+            };
+            float v;
+            int out;
+            if (a.gated) {
+                const int pair = r / 16;
+                v = total(pair * 32 + r % 16);
+                v = v / (1.0f + expf(-v)) * total(pair * 32 + 16 + r % 16);
+                out = (tile / 2 + pair) * 16 + r % 16;
+            } else {
+                v = total(r);
+                out = tile * 16 + r;
+            }
+            if (out < a.outputs) store_as(a.y, (long long)slot * a.outputs + out, v, a.dtype);
+        }
+    }
 }
 
 // y[t] = sum over s of w[t][s] * part[t * k + s], s ascending.
 template <class T> __global__ void __launch_bounds__(256) experts_sum_kernel(const float* part, const int* idx, const float* w, T* y, int k, int d, int E) {
     const int n = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+    wait_predecessor_grid();
     if (n >= d) return;
     float v = 0.0f;
     for (int s = 0; s < k; ++s) {
@@ -66,8 +409,6 @@ template <class T> __global__ void __launch_bounds__(256) experts_sum_kernel(con
     y[(long long)t * d + n] = from_f32<T>(v);
 }
 
-constexpr int kMaxRows = 512;
-
 }  // namespace
 }  // namespace moe
 
@@ -75,34 +416,51 @@ using namespace moe;
 
 struct MoeW4 {
     MoeW4Config cfg;
-    int outputs = 0, groups = 0;
-    uint8_t* codes = nullptr;
-    __half* scales = nullptr;
-    uint8_t* zeros = nullptr;
-    float* work = nullptr;    // this matrix's fp32 results of the experts: [work_rows][outputs]
+    int outputs = 0, tiles = 0, blocks = 0;
+    uint8_t* records = nullptr;
+    Planes x{};               // the activations' operand, of work_rows rows
+    float* result = nullptr;  // fp32 results of the experts: [work_rows][outputs]
     int work_rows = 0;
-    size_t bytes = 0;
+    size_t bytes = 0, work_bytes = 0;
 };
 
 namespace {
 
+void free_work(MoeW4* h) {
+    cudaFree(h->x.plane);
+    cudaFree(h->x.sums);
+    cudaFree(h->x.unit);
+    cudaFree(h->result);
+    h->x = Planes{};
+    h->result = nullptr;
+    h->bytes -= h->work_bytes;
+    h->work_bytes = 0;
+    h->work_rows = 0;
+}
+
 int ensure_rows(MoeW4* h, int rows) {
     if (rows <= h->work_rows) return MOE_OK;
-    float* p = nullptr;
-    const size_t n = (size_t)rows * h->outputs * sizeof(float);
-    if (cudaMalloc(&p, n) != cudaSuccess) {
+    free_work(h);   // waits for what still uses it
+    const size_t plane = (size_t)rows * 2 * h->blocks * 256, unit = rows * sizeof(float);
+    const size_t sums = (size_t)rows * h->blocks * (kBlockK / h->cfg.group) * sizeof(float);
+    const size_t result = (size_t)rows * h->outputs * sizeof(float);
+    cudaError_t e = cudaMalloc(&h->x.plane, plane);
+    if (e == cudaSuccess) e = cudaMalloc(&h->x.sums, sums);
+    if (e == cudaSuccess) e = cudaMalloc(&h->x.unit, unit);
+    if (e == cudaSuccess) e = cudaMalloc(&h->result, result);
+    if (e != cudaSuccess) {
         cudaGetLastError();
+        free_work(h);
         return report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed");
     }
-    cudaFree(h->work);
-    h->bytes += n - (size_t)h->work_rows * h->outputs * sizeof(float);
-    h->work = p;
+    h->work_bytes = plane + sums + unit + result;
+    h->bytes += h->work_bytes;
     h->work_rows = rows;
     return MOE_OK;
 }
 
 int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, const uint8_t* zeros, MoeW4** out,
-              cudaMemcpyKind kind) {
+              bool on_host) {
     if (!cfg || !codes || !scales || !out) return report_error(MOE_ERR_INVALID, "moe_w4_create: null argument");
     *out = nullptr;
     if (cfg->num_matrices < 1 || cfg->num_matrices > 256)
@@ -118,34 +476,56 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     int ndev = 0;
     if (cudaGetDeviceCount(&ndev) != cudaSuccess || cfg->device < 0 || cfg->device >= ndev)
         return report_error(MOE_ERR_INVALID, "moe_w4_create: no such device");
+    if (!on_host && (!aligned_to(codes, 4) || !aligned_to(scales, 2)))
+        return report_error(MOE_ERR_INVALID, "moe_w4_create: device codes must be 4-byte aligned, scales to their elements");
     OnDevice on(cfg->device);
     int major = 0;
     cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, cfg->device);
-    if (e != cudaSuccess || !on.ok) return launch_status(e, "moe_w4_create");
+    if (e != cudaSuccess) return launch_status(e, "moe_w4_create");
+    if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_create: cannot select the device");
     if (major != 10) return report_error(MOE_ERR_UNSUPPORTED, "libmoe_b200 is built for sm_100a (B200) only");
     auto* h = new MoeW4;
     h->cfg = *cfg;
     h->outputs = cfg->gated ? cfg->rows / 2 : cfg->rows;
-    h->groups = (cfg->cols + cfg->group - 1) / cfg->group;
-    const size_t rows = (size_t)cfg->num_matrices * cfg->rows;
-    const size_t nc = rows * (cfg->cols / 2), ng = rows * h->groups;
-    e = cudaMalloc(&h->codes, nc);
-    if (e == cudaSuccess) e = cudaMalloc(&h->scales, ng * 2);
-    if (e == cudaSuccess && zeros) e = cudaMalloc(&h->zeros, ng);
+    // Whole quads of tiles, so that a block of any tile count stays inside.
+    h->tiles = ((h->outputs + 15) / 16 * (cfg->gated ? 2 : 1) + 3) / 4 * 4;
+    h->blocks = (cfg->cols + kBlockK - 1) / kBlockK;
+    const int per = kBlockK / cfg->group, groups = (cfg->cols + cfg->group - 1) / cfg->group;
+    const size_t matrix = (size_t)h->tiles * h->blocks * w4_record(per), E = cfg->num_matrices;
+    e = cudaMalloc(&h->records, matrix * E);
     if (e != cudaSuccess) {
         cudaGetLastError();
-        moe_w4_destroy(h);
+        delete h;
         return report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed");
     }
-    e = cudaDeviceSynchronize();   // device sources may still be written on any stream
-    if (e == cudaSuccess) e = cudaMemcpy(h->codes, codes, nc, kind);
-    if (e == cudaSuccess) e = cudaMemcpy(h->scales, scales, ng * 2, kind);
-    if (e == cudaSuccess && zeros) e = cudaMemcpy(h->zeros, zeros, ng, kind);
+    h->bytes = matrix * E;
+    // Host weights pass through the device one matrix at a time.
+    const size_t nc = (size_t)cfg->rows * (cfg->cols / 2), ng = (size_t)cfg->rows * groups;
+    uint8_t* stage = nullptr;
+    const size_t scales_at = (nc + 15) / 16 * 16, zeros_at = scales_at + (ng * 2 + 15) / 16 * 16;
+    if (on_host) e = cudaMalloc(&stage, zeros_at + ng);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();   // device sources may still be written on any stream
+    for (size_t m = 0; m < E && e == cudaSuccess; ++m) {
+        PackArgs a{codes + m * nc, static_cast<const __half*>(scales) + m * ng, zeros ? zeros + m * ng : nullptr,
+                   h->records + m * matrix, cfg->rows, cfg->cols, cfg->group, h->tiles, h->blocks, cfg->gated != 0};
+        if (on_host) {
+            e = cudaMemcpy(stage, a.codes, nc, cudaMemcpyHostToDevice);
+            if (e == cudaSuccess) e = cudaMemcpy(stage + scales_at, a.scales, ng * 2, cudaMemcpyHostToDevice);
+            if (e == cudaSuccess && zeros) e = cudaMemcpy(stage + zeros_at, a.zeros, ng, cudaMemcpyHostToDevice);
+            a.codes = stage;
+            a.scales = reinterpret_cast<const __half*>(stage + scales_at);
+            a.zeros = zeros ? stage + zeros_at : nullptr;
+        }
+        if (e == cudaSuccess)
+            e = launch(w4_pack_kernel, dim3((unsigned)((long long)h->tiles * h->blocks)), 256, 0, nullptr, false, a);
+    }
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
-    h->bytes = nc + ng * (zeros ? 3 : 2);
-    int rc = launch_status(e, "moe_w4_create");
+    cudaFree(stage);
+    int rc = e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed")
+                                            : launch_status(e, "moe_w4_create");
     if (rc == MOE_OK) rc = ensure_rows(h, cfg->max_rows);
     if (rc != MOE_OK) {
+        cudaGetLastError();
         moe_w4_destroy(h);
         return rc;
     }
@@ -153,21 +533,40 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     return MOE_OK;
 }
 
-template <class TX, class TY>
-cudaError_t matvec_typed(const MoeW4* h, const void* x, int rows, int64_t x_stride, int x_share, const int* matrix,
-                         void* y, cudaStream_t s) {
-    W4Args a{h->codes, h->scales, h->zeros, x, matrix, y, x_stride, rows, x_share, h->cfg.num_matrices, h->cfg.rows,
-             h->cfg.cols, h->cfg.group, h->outputs, h->cfg.gated != 0};
-    return launch(matvec_kernel<TX, TY>, dim3((h->outputs + 7) / 8, rows), 256, 0, s, false, a);
+template <int kPlanes, int MT, int NT>
+cudaError_t product_groups(const MoeW4* h, const MatvecArgs& a, cudaStream_t s) {
+    const dim3 grid((a.tiles + MT - 1) / MT, a.matrix ? a.E : 1), block(kWarps * 32);
+    switch (kBlockK / h->cfg.group) {
+        case 1: return launch(w4_matvec_kernel<kPlanes, MT, NT, 1>, grid, block, 0, s, true, a);
+        case 2: return launch(w4_matvec_kernel<kPlanes, MT, NT, 2>, grid, block, 0, s, true, a);
+        default: return launch(w4_matvec_kernel<kPlanes, MT, NT, 4>, grid, block, 0, s, true, a);
+    }
 }
 
 template <class T>
-cudaError_t experts_typed(MoeW4* gu, MoeW4* dn, const void* x, int T_, int k, const int* idx, const float* w, void* y,
-                          cudaStream_t s) {
-    cudaError_t e = matvec_typed<T, float>(gu, x, T_ * k, gu->cfg.cols, k, idx, gu->work, s);
-    if (e == cudaSuccess) e = matvec_typed<float, float>(dn, gu->work, T_ * k, dn->cfg.cols, 1, idx, dn->work, s);
+cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, int x_share, const int* matrix, void* y,
+                    int dtype, bool dependent, cudaStream_t s) {
+    constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
+    const MoeW4Config& c = h->cfg;
+    const int x_rows = (num_rows + x_share - 1) / x_share;
+    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 512, 0, s, dependent, x, (long long)x_stride, c.cols,
+                           h->blocks, c.group, h->x);
     if (e != cudaSuccess) return e;
-    return launch(experts_sum_kernel<T>, dim3((dn->outputs + 255) / 256, T_), 256, 0, s, false, dn->work, idx, w,
+    MatvecArgs a{h->records, h->x, matrix, y, num_rows, x_share, c.num_matrices, h->tiles, h->blocks, h->outputs, dtype,
+                 c.gated != 0};
+    const int columns = num_rows * kPlanes;
+    return columns <= 8 ? product_groups<kPlanes, 2, 1>(h, a, s) : product_groups<kPlanes, 4, 2>(h, a, s);
+}
+
+template <class T>
+cudaError_t experts_typed(MoeW4* gu, MoeW4* dn, const void* x, int tokens, int k, const int* idx, const float* w, void* y,
+                          cudaStream_t s) {
+    cudaError_t e = product(gu, static_cast<const T*>(x), tokens * k, gu->cfg.cols, k, idx, gu->result, MOE_DTYPE_F32,
+                            false, s);
+    if (e == cudaSuccess)
+        e = product(dn, gu->result, tokens * k, dn->cfg.cols, 1, idx, dn->result, MOE_DTYPE_F32, true, s);
+    if (e != cudaSuccess) return e;
+    return launch(experts_sum_kernel<T>, dim3((dn->outputs + 255) / 256, tokens), 256, 0, s, true, dn->result, idx, w,
                   static_cast<T*>(y), k, dn->outputs, dn->cfg.num_matrices);
 }
 
@@ -187,22 +586,20 @@ void moe_w4_config_init(MoeW4Config* c) {
 
 int moe_w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, const uint8_t* zeros,
                   MoeW4** out) {
-    return guarded("moe_w4_create", [&] { return w4_create(cfg, codes, scales, zeros, out, cudaMemcpyHostToDevice); });
+    return guarded("moe_w4_create", [&] { return w4_create(cfg, codes, scales, zeros, out, true); });
 }
 
 int moe_w4_create_from_device(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, const uint8_t* zeros,
                               MoeW4** out) {
     return guarded("moe_w4_create_from_device",
-                   [&] { return w4_create(cfg, codes, scales, zeros, out, cudaMemcpyDeviceToDevice); });
+                   [&] { return w4_create(cfg, codes, scales, zeros, out, false); });
 }
 
 void moe_w4_destroy(MoeW4* h) {
     if (!h) return;
     OnDevice on(h->cfg.device);
-    cudaFree(h->codes);
-    cudaFree(h->scales);
-    cudaFree(h->zeros);
-    cudaFree(h->work);
+    cudaFree(h->records);
+    free_work(h);
     delete h;
 }
 
@@ -222,13 +619,15 @@ int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_row
         OnDevice on(h->cfg.device);
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_matvec_device: cannot select the device");
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const int rc = ensure_rows(h, num_rows);
+        if (rc != MOE_OK) return rc;
         cudaError_t e;
         if (dtype == MOE_DTYPE_F32)
-            e = matvec_typed<float, float>(h, x, num_rows, x_row_stride, x_share, matrix, y, s);
+            e = product(h, static_cast<const float*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, s);
         else if (dtype == MOE_DTYPE_BF16)
-            e = matvec_typed<__nv_bfloat16, __nv_bfloat16>(h, x, num_rows, x_row_stride, x_share, matrix, y, s);
+            e = product(h, static_cast<const __nv_bfloat16*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, s);
         else
-            e = matvec_typed<__half, __half>(h, x, num_rows, x_row_stride, x_share, matrix, y, s);
+            e = product(h, static_cast<const __half*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, s);
         return launch_status(e, "moe_w4_matvec_device");
     });
 }

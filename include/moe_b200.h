@@ -656,7 +656,8 @@ size_t moe_w4_device_bytes(const MoeW4* h);
  * [num_rows][outputs] contiguous, both of `dtype`.  matrix [num_rows] (device,
  * may be null: matrix 0): the matrix of each product; a row whose entry is
  * outside [0, num_matrices) gets zeros.  Sums are in fp32; x enters the
- * products exactly. */
+ * products as float16 scaled by a power of two per row: 16-bit types exactly
+ * (to 2^-34 of the row's largest), fp32 with 22 significant bits. */
 int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_rows,
                          int64_t x_row_stride, int32_t x_share, const int32_t* matrix, void* y,
                          void* stream);
@@ -667,8 +668,7 @@ int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_row
  * outputs == down's cols, both with the same num_matrices; x and y
  * [num_tokens][gate_up cols / down rows] contiguous of `dtype`, idx and
  * weights [num_tokens][top_k] as moe_route_device writes them.
- * num_tokens * top_k <= 512.  The hidden activations are kept in fp32 and
- * enter the down product exactly. */
+ * num_tokens * top_k <= 512.  The hidden activations are kept in fp32. */
 int moe_w4_experts_device(MoeW4* gate_up, MoeW4* down, const void* x, int32_t dtype,
                           int32_t num_tokens, int32_t top_k, const int32_t* idx,
                           const float* weights, void* y, void* stream);
