@@ -1,5 +1,6 @@
 // Matrix-vector products with 4-bit group-scaled weights, and the routed
 // experts built on them.
+#include <algorithm>
 #include <cstring>
 #include <new>
 
@@ -13,7 +14,10 @@ namespace {
 
 constexpr int kMaxRows = 512;        // products of one call
 constexpr int kBlockK = 128;         // columns of a record
-constexpr int kWarps = 8;
+constexpr int kMaxMatrices = 256;
+// Threads of a block and blocks of an SM, by column tiles: registers.
+__host__ __device__ constexpr int w4_threads(int NT) { return NT == 1 ? 256 : 128; }
+__host__ __device__ constexpr int w4_blocks(int NT) { return NT == 1 ? 2 : 3; }
 
 // The handle's own layout of the weights: records of 16 rows x 128 columns,
 // [matrix][tile of 16 rows][block of 128 columns].  Lane 4 g + j of a warp
@@ -134,8 +138,9 @@ struct MatvecArgs {
     Planes x;
     const int* matrix;      // [num_rows], or null
     void* y;                // [num_rows][outputs]
-    int num_rows, x_share, E, tiles, blocks, outputs, dtype;
+    int num_rows, x_share, E, tiles, groups, blocks, outputs, dtype;   // groups: items of a matrix
     bool gated;
+    int tiles_used;         // tiles with rows of the matrix
 };
 
 __device__ __forceinline__ uint4 load_stream(const uint4* p) {
@@ -151,105 +156,159 @@ __device__ __forceinline__ void store_as(void* y, long long at, float v, int dty
     else static_cast<__half*>(y)[at] = from_f32<__half>(v);
 }
 
-// y = W x for the rows of x that ask for one matrix; a block has MT tiles of 16
-// weight rows, its warps every eighth block of 128 columns.
+// Which products ask for which matrix: the matrices in use in ascending order,
+// each with its products in ascending order.
+struct Sorted {
+    short rows[kMaxRows];           // products, sorted by matrix
+    short first[kMaxMatrices + 1];  // [used + 1] into rows
+    short matrix[kMaxMatrices];     // [used]
+    short of[kMaxRows];             // matrix of each product, -1 outside the range
+    short count[kMaxMatrices];
+    int used;
+};
+
+// Called by all threads of the block.
+template <int kThreads> __device__ void sort_products(Sorted& s, const int* matrix, int n, int E) {
+    if (!matrix) {
+        for (int i = threadIdx.x; i < n; i += kThreads) s.rows[i] = (short)i;
+        if (threadIdx.x == 0) {
+            s.used = 1;
+            s.matrix[0] = s.first[0] = 0;
+            s.first[1] = (short)n;
+        }
+        __syncthreads();
+        return;
+    }
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int e = __ldg(matrix + i);
+        s.of[i] = (short)(e >= 0 && e < E ? e : -1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kThreads) {
+        int c = 0;
+        for (int i = 0; i < n; ++i) c += s.of[i] == e;
+        s.count[e] = (short)c;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int used = 0, at = 0;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + threadIdx.x, c = e < E ? s.count[e] : 0;
+            int sum = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (threadIdx.x >= o) sum += v;
+            }
+            const unsigned m = __ballot_sync(0xffffffffu, c > 0);
+            if (c > 0) {
+                const int k = used + __popc(m & ((1u << threadIdx.x) - 1));
+                s.matrix[k] = (short)e;
+                s.first[k] = (short)(at + sum - c);
+                s.count[e] = (short)(at + sum - c);     // from here on the place of its first product
+            }
+            used += __popc(m);
+            at += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (threadIdx.x == 0) {
+            s.used = used;
+            s.first[used] = (short)at;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int e = s.of[i];
+        if (e < 0) continue;
+        int rank = 0;
+        for (int k = 0; k < i; ++k) rank += s.of[k] == e;
+        s.rows[s.count[e] + rank] = (short)i;
+    }
+    __syncthreads();
+}
+
+// y = W x.  An item is (matrix in use, MT tiles of 16 weight rows); the blocks
+// take the items in turn, a warp every kWarps-th block of 128 columns.
 //
 // Bound by reading the weights, so a warp streams its records straight into
-// registers, kDepth of them ahead (the first ones before the activations'
-// kernel has ended), and no weight passes through shared memory.  Products:
-// m16n8k16 with the codes as A and up to 8 NT columns of activations (a row of
-// x, or one of its two planes) as B.  A 4-bit code in the low bits of a
-// float16 word is the subnormal c 2^-24 (c 2^-20 four bits higher): one AND
-// makes an operand of two codes.  With one plane the zero is taken off after
-// the group's sum, s (sum(c x) - z sum(x)); with two (fp32), where the sum's
-// last bits count, code and zero become the normal number (c - z) 2^-10 by one
-// fma.  The warps' sums are added in order through shared memory.
+// registers, four of them ahead (the first ones before the activations' kernel
+// has ended, the next item's before this one's sums are joined), and no weight
+// passes through shared memory.  Products: m16n8k16 with the codes as A and up
+// to 8 NT columns of activations (a row of x, or one of its two planes) as B.
+// A 4-bit code in the low bits of a float16 word is the subnormal c 2^-24
+// (c 2^-20 four bits higher): one AND makes an operand of two codes.  With one
+// plane the zero is taken off after the group's sum, s (sum(c x) - z sum(x));
+// with two (fp32), where the sum's last bits count, code and zero become the
+// normal number (c - z) 2^-10 by one fma.  The warps' sums are added in order
+// through shared memory.
 template <int kPlanes, int MT, int NT, int kPer>
-__global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel(MatvecArgs a) {
-    constexpr int kCols = 8 * NT, kTokens = kCols / kPlanes;     // products per pass
+__global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kernel(MatvecArgs a) {
+    constexpr int kThreads = w4_threads(NT), kWarps = kThreads / 32;
+    constexpr int kTokens = 8 * NT / kPlanes;                    // products per pass
     constexpr int kV = kPlanes == 2 ? 2 : 4;                     // sums per lane, tile and column tile
-    constexpr int kDepth = 2;
+    constexpr int kDepth = 4 / MT, kUnroll = kDepth < 2 ? 2 : kDepth;
     constexpr int kRecord = w4_record(kPer);
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     __shared__ float part[kWarps][MT * 16][kTokens + 1];
-    __shared__ short list[kMaxRows];
-    __shared__ int list_n;
+    __shared__ Sorted sorted;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-    const int tile = blockIdx.x * MT;
-
-    // The products that ask for this block's matrix, in order.
-    int matrix = 0, n = a.num_rows;
-    if (a.matrix) {
-        matrix = blockIdx.y;
-        if (warp == 0) {
-            int count = 0;
-            for (int i = 0; i < a.num_rows; i += 32) {
-                const bool mine = i + lane < a.num_rows && __ldg(a.matrix + i + lane) == matrix;
-                const unsigned m = __ballot_sync(0xffffffffu, mine);
-                if (mine) list[count + __popc(m & ((1u << lane) - 1))] = (short)(i + lane);
-                count += __popc(m);
-            }
-            if (lane == 0) list_n = count;
-        }
-        __syncthreads();
-        n = list_n;
-        if (matrix == 0) {   // zeros for the products without a matrix
-            wait_predecessor_grid();
-            const int first = (a.gated ? tile / 2 : tile) * 16, rows = min(a.gated ? MT * 8 : MT * 16, a.outputs - first);
-            for (int i = warp; i < a.num_rows; i += kWarps) {
-                const int m = __ldg(a.matrix + i);
-                if (m >= 0 && m < a.E) continue;
-                for (int r = lane; r < rows; r += 32) store_as(a.y, (long long)i * a.outputs + first + r, 0.0f, a.dtype);
-            }
-        }
-        if (n == 0) return;
-    }
-    const uint8_t* base = a.records + ((long long)matrix * a.tiles + tile) * a.blocks * kRecord;
+    sort_products<kThreads>(sorted, a.matrix, a.num_rows, a.E);
+    const int items = sorted.used * a.groups;
     const long long tile_step = (long long)a.blocks * kRecord;
 
-    struct Raw {
-        uint4 code[MT][2];
-        uint32_t par[MT][2 * kPer];
+    uint4 code[kDepth][MT][2];
+    uint32_t par[kDepth][MT][2 * kPer];
+    const uint8_t* base = nullptr;     // the item's records, at the lane's place
+    auto begin = [&](int item) {
+        const int m = item / a.groups, tile = (item - m * a.groups) * MT;
+        base = a.records + ((long long)sorted.matrix[m] * a.tiles + tile) * tile_step + lane * 16;
     };
-    Raw raw[kDepth];
-    auto fetch = [&](Raw& r, int kb) {
+    auto fetch = [&](int d, int t, int kb) {
         if (kb < a.blocks) {
+            const uint8_t* rec = base + t * tile_step + (long long)kb * kRecord;
+            code[d][t][0] = load_stream(reinterpret_cast<const uint4*>(rec));
+            code[d][t][1] = load_stream(reinterpret_cast<const uint4*>(rec + 512));
+            const uint8_t* p = rec - lane * 16 + 1024 + g * (8 * kPer);
+            if constexpr (kPer == 1) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                par[d][t][0] = v.x, par[d][t][1] = v.y;
+            } else {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const uint8_t* rec = base + t * tile_step + (long long)kb * kRecord;
-                r.code[t][0] = load_stream(reinterpret_cast<const uint4*>(rec) + lane);
-                r.code[t][1] = load_stream(reinterpret_cast<const uint4*>(rec + 512) + lane);
-                const uint8_t* p = rec + 1024 + g * (8 * kPer);
-                if constexpr (kPer == 1) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-                    r.par[t][0] = v.x, r.par[t][1] = v.y;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2 * kPer; i += 4) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
-                        r.par[t][i] = v.x, r.par[t][i + 1] = v.y, r.par[t][i + 2] = v.z, r.par[t][i + 3] = v.w;
-                    }
+                for (int i = 0; i < 2 * kPer; i += 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+                    par[d][t][i] = v.x, par[d][t][i + 1] = v.y, par[d][t][i + 2] = v.z, par[d][t][i + 3] = v.w;
                 }
             }
         }
     };
-
-    for (int t0 = 0; t0 < n; t0 += kTokens) {
+    auto fetch_first = [&]() {
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) fetch(raw[d], warp + d * kWarps);
-        if (t0 == 0) {
-            wait_predecessor_grid();
-            launch_dependents();
-        }
+        for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) fetch(d, t, warp + d * kWarps);
+    };
+    int item = blockIdx.x, t0 = 0;
+    if (item < items) {
+        begin(item);
+        fetch_first();
+    }
+    wait_predecessor_grid();
+    launch_dependents();
+    if (a.matrix) {   // zeros for the products without a matrix
+        for (int i = blockIdx.x * kWarps + warp; i < a.num_rows; i += gridDim.x * kWarps)
+            if (sorted.of[i] < 0)
+                for (int r = lane; r < a.outputs; r += 32) store_as(a.y, (long long)i * a.outputs + r, 0.0f, a.dtype);
+    }
+
+    while (item < items) {
+        const int m = item / a.groups, tile = (item - m * a.groups) * MT;
+        const short* rows = sorted.rows + sorted.first[m];
+        const int n = sorted.first[m + 1] - sorted.first[m];
         // The lane's column of B, and the rows whose sums it holds.
         const uint4* bx[NT];
         const float* sx[NT][2 / kPlanes];
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
-            auto x_row = [&](int token) {
-                const int i = min(t0 + token, n - 1);
-                return (a.matrix ? list[i] : i) / a.x_share;
-            };
+            auto x_row = [&](int token) { return rows[min(t0 + token, n - 1)] / a.x_share; };
             const int col = c * 8 + g, token = col / kPlanes;
             const long long per_row = (long long)a.blocks * 16;
             bx[c] = t0 + token < n ? a.x.plane + (x_row(token) * kPlanes + col % kPlanes) * per_row + j : nullptr;
@@ -257,18 +316,16 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
             for (int i = 0; i < 2 / kPlanes; ++i)
                 sx[c][i] = a.x.sums + (long long)x_row((c * 8 + 2 * j) / kPlanes + i) * a.blocks * kPer;
         }
-        uint4 bw[kDepth][NT][4];
+        uint4 bw[2][NT][4];
         auto fetch_x = [&](uint4 (&b)[NT][4], int kb) {
-            if (kb < a.blocks) {
 #pragma unroll
-                for (int c = 0; c < NT; ++c)
+            for (int c = 0; c < NT; ++c)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        b[c][w] = bx[c] ? __ldg(bx[c] + kb * 16 + w * 4) : make_uint4(0, 0, 0, 0);
-            }
+                for (int w = 0; w < 4; ++w)
+                    b[c][w] = bx[c] && kb < a.blocks ? __ldg(bx[c] + kb * 16 + w * 4) : make_uint4(0, 0, 0, 0);
         };
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) fetch_x(bw[d], warp + d * kWarps);
+        fetch_x(bw[0], warp);
+        fetch_x(bw[1], warp + kWarps);
 
         float y[MT][NT][kV];
 #pragma unroll
@@ -278,10 +335,10 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
 #pragma unroll
                 for (int i = 0; i < kV; ++i) y[t][c][i] = 0.0f;
 
-        for (int kb0 = warp; kb0 < a.blocks; kb0 += kDepth * kWarps) {
+        for (int kb0 = warp; kb0 < a.blocks; kb0 += kUnroll * kWarps) {
 #pragma unroll
-            for (int d = 0; d < kDepth; ++d) {
-                const int kb = kb0 + d * kWarps;
+            for (int d = 0; d < kUnroll; ++d) {
+                const int kb = kb0 + d * kWarps, slot = d % kDepth;
                 if (kb >= a.blocks) break;
                 float sums[NT][2][kPer];
                 if constexpr (kPlanes == 1) {
@@ -294,7 +351,7 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
                 }
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
-                    const uint4 c0 = raw[d].code[t][0], c1 = raw[d].code[t][1];
+                    const uint4 c0 = code[slot][t][0], c1 = code[slot][t][1];
                     const uint32_t lo[4] = {c0.x, c0.y, c0.z, c0.w}, hi[4] = {c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
                     for (int q = 0; q < kPer; ++q) {
@@ -303,7 +360,7 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
                         if constexpr (kPlanes == 2) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
-                                zero[h] = __hmul2(__high2half2(*reinterpret_cast<const __half2*>(&raw[d].par[t][h * kPer + q])),
+                                zero[h] = __hmul2(__high2half2(*reinterpret_cast<const __half2*>(&par[slot][t][h * kPer + q])),
                                                   __float2half2_rn(-1.0f / 1024.0f));
                         }
                         auto operand = [&](uint32_t word, uint32_t mask, int h) -> uint32_t {
@@ -324,7 +381,7 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
                                                        operand(l, kOdd, 0), operand(u, kOdd, 1)};
 #pragma unroll
                                 for (int c = 0; c < NT; ++c) {
-                                    const uint4 b = bw[d][c][w];
+                                    const uint4 b = bw[d % 2][c][w];
                                     const uint32_t b0 = half ? b.z : b.x, b1 = half ? b.w : b.y;
                                     if (w == q * (4 / kPer) && half == 0) mma_f16_first(acc[c], f, b0, b1);
                                     else mma_f16(acc[c], f, b0, b1);
@@ -332,7 +389,7 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
                             }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&raw[d].par[t][h * kPer + q]));
+                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&par[slot][t][h * kPer + q]));
 #pragma unroll
                             for (int c = 0; c < NT; ++c) {
                                 if constexpr (kPlanes == 2) {
@@ -348,12 +405,21 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
                             }
                         }
                     }
+                    fetch(slot, t, kb + kDepth * kWarps);
                 }
-                fetch(raw[d], kb + kDepth * kWarps);
-                fetch_x(bw[d], kb + kDepth * kWarps);
+                fetch_x(bw[d % 2], kb + 2 * kWarps);
             }
         }
-        __syncthreads();   // the last pass's sums are read
+        int next = item, next_t0 = t0 + kTokens;
+        if (next_t0 >= n) {
+            next = item + gridDim.x;
+            next_t0 = 0;
+        }
+        if (next < items) {
+            begin(next);
+            fetch_first();
+        }
+        __syncthreads();   // the last item's sums are read
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -370,10 +436,10 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
         __syncthreads();
         const int now = min(kTokens, n - t0);
         const int out_rows = a.gated ? MT * 8 : MT * 16;
-        for (int i = threadIdx.x; i < out_rows * now; i += kWarps * 32) {
+        for (int i = threadIdx.x; i < out_rows * now; i += kThreads) {
             const int r = i % out_rows, token = i / out_rows;
-            const int slot = a.matrix ? list[t0 + token] : t0 + token;
-            const float unit = __ldg(a.x.unit + slot / a.x_share) * (kPlanes == 2 ? 1024.0f : 1.0f);
+            const int product = rows[t0 + token];
+            const float unit = __ldg(a.x.unit + product / a.x_share) * (kPlanes == 2 ? 1024.0f : 1.0f);
             auto total = [&](int row) {
                 float v = 0.0f;
 #pragma unroll
@@ -391,8 +457,10 @@ __global__ void __launch_bounds__(kWarps * 32, MT == 4 ? 1 : 2) w4_matvec_kernel
                 v = total(r);
                 out = tile * 16 + r;
             }
-            if (out < a.outputs) store_as(a.y, (long long)slot * a.outputs + out, v, a.dtype);
+            if (out < a.outputs) store_as(a.y, (long long)product * a.outputs + out, v, a.dtype);
         }
+        item = next;
+        t0 = next_t0;
     }
 }
 
@@ -416,7 +484,7 @@ using namespace moe;
 
 struct MoeW4 {
     MoeW4Config cfg;
-    int outputs = 0, tiles = 0, blocks = 0;
+    int outputs = 0, tiles = 0, blocks = 0, sms = 0;
     uint8_t* records = nullptr;
     Planes x{};               // the activations' operand, of work_rows rows
     float* result = nullptr;  // fp32 results of the experts: [work_rows][outputs]
@@ -479,13 +547,15 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     if (!on_host && (!aligned_to(codes, 4) || !aligned_to(scales, 2)))
         return report_error(MOE_ERR_INVALID, "moe_w4_create: device codes must be 4-byte aligned, scales to their elements");
     OnDevice on(cfg->device);
-    int major = 0;
+    int major = 0, sms = 0;
     cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, cfg->device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cfg->device);
     if (e != cudaSuccess) return launch_status(e, "moe_w4_create");
     if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_create: cannot select the device");
     if (major != 10) return report_error(MOE_ERR_UNSUPPORTED, "libmoe_b200 is built for sm_100a (B200) only");
     auto* h = new MoeW4;
     h->cfg = *cfg;
+    h->sms = sms;
     h->outputs = cfg->gated ? cfg->rows / 2 : cfg->rows;
     // Whole quads of tiles, so that a block of any tile count stays inside.
     h->tiles = ((h->outputs + 15) / 16 * (cfg->gated ? 2 : 1) + 3) / 4 * 4;
@@ -534,8 +604,9 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
 }
 
 template <int kPlanes, int MT, int NT>
-cudaError_t product_groups(const MoeW4* h, const MatvecArgs& a, cudaStream_t s) {
-    const dim3 grid((a.tiles + MT - 1) / MT, a.matrix ? a.E : 1), block(kWarps * 32);
+cudaError_t launch_product(const MoeW4* h, MatvecArgs a, int used, cudaStream_t s) {
+    a.groups = (a.tiles_used + MT - 1) / MT;
+    const dim3 grid((unsigned)std::min((long long)a.groups * used, (long long)h->sms * w4_blocks(NT))), block(w4_threads(NT));
     switch (kBlockK / h->cfg.group) {
         case 1: return launch(w4_matvec_kernel<kPlanes, MT, NT, 1>, grid, block, 0, s, true, a);
         case 2: return launch(w4_matvec_kernel<kPlanes, MT, NT, 2>, grid, block, 0, s, true, a);
@@ -552,10 +623,17 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 512, 0, s, dependent, x, (long long)x_stride, c.cols,
                            h->blocks, c.group, h->x);
     if (e != cudaSuccess) return e;
-    MatvecArgs a{h->records, h->x, matrix, y, num_rows, x_share, c.num_matrices, h->tiles, h->blocks, h->outputs, dtype,
-                 c.gated != 0};
-    const int columns = num_rows * kPlanes;
-    return columns <= 8 ? product_groups<kPlanes, 2, 1>(h, a, s) : product_groups<kPlanes, 4, 2>(h, a, s);
+    MatvecArgs a{h->records, h->x, matrix, y, num_rows, x_share, matrix ? c.num_matrices : 1, h->tiles, 0, h->blocks,
+                 h->outputs, dtype, c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
+    // Columns of a matrix's products: all rows', or twice the mean's where the rows choose their matrices.
+    const int columns = kPlanes * (matrix ? std::min(num_rows, 2 * ((num_rows + c.num_matrices - 1) / c.num_matrices)) : num_rows);
+    const int used = matrix ? std::min(num_rows, c.num_matrices) : 1;
+    const long long work = (long long)a.tiles_used * used;
+    if (columns <= 8)
+        return work >= 16ll * h->sms              ? launch_product<kPlanes, 4, 1>(h, a, used, s)
+               : work >= 3ll * h->sms || c.gated ? launch_product<kPlanes, 2, 1>(h, a, used, s)
+                                                  : launch_product<kPlanes, 1, 1>(h, a, used, s);
+    return launch_product<kPlanes, 2, 2>(h, a, used, s);
 }
 
 template <class T>
