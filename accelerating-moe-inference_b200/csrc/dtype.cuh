@@ -26,6 +26,21 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^s >= d the
+// smallest such power, q = floor(n m / 2^(31 + s)) for m = ceil(2^(31 + s) / d),
+// since n (m d - 2^(31 + s)) < 2^31 d <= 2^(31 + s).
+struct FastDiv {
+    unsigned long long mul;
+    int shift, d;
+    FastDiv() = default;
+    explicit FastDiv(int div) : d(div) {
+        shift = 31;
+        while ((1ll << (shift - 31)) < div) ++shift;
+        mul = ((1ull << shift) + div - 1) / div;
+    }
+    __device__ __forceinline__ int div(int n) const { return (int)((unsigned)n * mul >> shift); }
+};
+
 inline bool valid_dtype(int32_t t) { return t >= MOE_DTYPE_F32 && t <= MOE_DTYPE_F16; }
 inline size_t dtype_bytes(int32_t t) { return t == MOE_DTYPE_F32 ? 4 : 2; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

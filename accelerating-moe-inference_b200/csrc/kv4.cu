@@ -267,21 +267,6 @@ template <class T, int D, bool kVec> __global__ void __launch_bounds__(256) appe
 }
 
 // -------------------------------------------------------------- attention
-// n / d for 0 <= n < 2^31 by a multiplication: with 2^s >= d the
-// smallest such power, q = floor(n m / 2^(31 + s)) for m = ceil(2^(31 + s) / d),
-// since n (m d - 2^(31 + s)) < 2^31 d <= 2^(31 + s).
-struct FastDiv {
-    unsigned long long mul;
-    int shift, d;
-    FastDiv() = default;
-    explicit FastDiv(int div) : d(div) {
-        shift = 31;
-        while ((1ll << (shift - 31)) < div) ++shift;
-        mul = ((1ull << shift) + div - 1) / div;
-    }
-    __device__ __forceinline__ int div(int n) const { return (int)((unsigned)n * mul >> shift); }
-};
-
 struct AttendArgs {
     const uint8_t* cache;
     const void* q;

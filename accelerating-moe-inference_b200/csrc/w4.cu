@@ -20,7 +20,7 @@ __host__ __device__ constexpr int w4_threads(int NT) { return NT == 1 ? 256 : 12
 __host__ __device__ constexpr int w4_blocks(int NT) { return NT == 1 ? 2 : 3; }
 
 // The handle's own layout of the weights: records of 16 rows x 128 columns,
-// [matrix][tile of 16 rows][block of 128 columns].  Lane 4 g + j of a warp
+// [matrix][quad of tiles of 16 rows][block of 128 columns][4 tiles].  Lane 4 g + j of a warp
 // owns, of rows g and g + 8, the columns 32 w + 8 j .. + 7 of each w < 4:
 //   codes   [row half][lane][4 w] 32-bit words, the lowest nibble first
 //   params  [8 g][row half][128 / group] (scale, zero) float16 pairs
@@ -43,7 +43,7 @@ struct PackArgs {
 __global__ void __launch_bounds__(256) w4_pack_kernel(PackArgs a) {
     const int block = blockIdx.x % a.blocks, tile = blockIdx.x / a.blocks, per = kBlockK / a.group;
     const long long matrix = blockIdx.y;
-    uint8_t* rec = a.out + ((matrix * a.tiles + tile) * a.blocks + block) * w4_record(per);
+    uint8_t* rec = a.out + ((matrix * (a.tiles / 4) + tile / 4) * a.blocks + block) * (4 * w4_record(per)) + tile % 4 * w4_record(per);
     const int half_rows = a.gated ? a.rows / 2 : a.rows;
     auto row_of = [&](int r) {      // source row of the tile's row r, -1 for padding
         const int at = (a.gated ? tile >> 1 : tile) * 16 + r;
@@ -71,110 +71,32 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(PackArgs a) {
     }
 }
 
-// ------------------------------------------------------------ activations
-// A row of activations as the products' operand: scaled by a power of two to
-// below 2^11, as one float16 plane (16-bit types: exact down to 2^-34 of the
-// row's largest) or two, hi and (x - hi) 2^11 (fp32: 22 bits).
-//   plane   [row][plane][block of 128][4 w][4 j] 16 bytes: the float16 pairs
-//           (i, i + 4), i < 4, of columns 32 w + 8 j .. + 7; with one plane
-//           those of even i times 16 to match their codes' 2^-24
-//   sums    [row][blocks * 128 / group] of the scaled values
-//   unit    [row] what a scaled sum is multiplied by
-struct Planes {
-    uint4* plane;
-    float* sums;
-    float* unit;
-};
-
-template <class T, int kPlanes>
-__global__ void __launch_bounds__(512) w4_planes_kernel(const T* x, long long stride, int cols, int blocks, int group, Planes out) {
-    __shared__ float best[16];
-    const int row = blockIdx.x;
-    const T* p = x + row * stride;
-    wait_predecessor_grid();
-    launch_dependents();
-    float mx = 0.0f;
-    for (int k = threadIdx.x; k < cols; k += 512) mx = fmaxf(mx, fabsf(to_f32(p[k])));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mx;
-    __syncthreads();
-    mx = best[threadIdx.x & 15];
-#pragma unroll
-    for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    // Exponent of the largest, kept where 2^(10 - e) is a normal number.
-    const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
-    const float up = __uint_as_float((264 - e) << 23);
-    if (threadIdx.x == 0) out.unit[row] = __uint_as_float((e - 10) << 23);
-    const int chunks = blocks * (kBlockK / 8), per = group / 8;
-    for (int c = threadIdx.x; c < chunks; c += 512) {    // chunks is a multiple of 16: whole groups of lanes
-        float v[8], sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += v[i] = c * 8 < cols ? to_f32(p[c * 8 + i]) * up : 0.0f;
-        const unsigned live = __activemask();
-        for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
-        if (c % per == 0) out.sums[(long long)row * (chunks / per) + c / per] = sum;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float f = kPlanes == 2 || (i & 1) ? 1.0f : 16.0f;
-            const __half2 h = __floats2half2_rn(v[i] * f, v[i + 4] * f);
-            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-            if constexpr (kPlanes == 2) {
-                const float2 b = __half22float2(h);
-                const __half2 l = __floats2half2_rn((v[i] * f - b.x) * 2048.0f, (v[i + 4] * f - b.y) * 2048.0f);
-                lo[i] = *reinterpret_cast<const uint32_t*>(&l);
-            }
-        }
-        uint4* to = out.plane + (long long)row * kPlanes * chunks + c;
-        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (kPlanes == 2) to[chunks] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-}
-
-// --------------------------------------------------------------- products
-struct MatvecArgs {
-    const uint8_t* records;
-    Planes x;
-    const int* matrix;      // [num_rows], or null
-    void* y;                // [num_rows][outputs]
-    int num_rows, x_share, E, tiles, groups, blocks, outputs, dtype;   // groups: items of a matrix
-    bool gated;
-    int tiles_used;         // tiles with rows of the matrix
-};
-
-__device__ __forceinline__ uint4 load_stream(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-
-__device__ __forceinline__ void store_as(void* y, long long at, float v, int dtype) {
-    if (dtype == MOE_DTYPE_F32) static_cast<float*>(y)[at] = v;
-    else if (dtype == MOE_DTYPE_BF16) static_cast<__nv_bfloat16*>(y)[at] = from_f32<__nv_bfloat16>(v);
-    else static_cast<__half*>(y)[at] = from_f32<__half>(v);
-}
-
 // Which products ask for which matrix: the matrices in use in ascending order,
-// each with its products in ascending order.
+// each with its products in ascending order.  A matrix's products fill column
+// tiles of 8, kPlanes columns each.
 struct Sorted {
     short rows[kMaxRows];           // products, sorted by matrix
     short first[kMaxMatrices + 1];  // [used + 1] into rows
     short matrix[kMaxMatrices];     // [used]
     short of[kMaxRows];             // matrix of each product, -1 outside the range
-    short count[kMaxMatrices];
+    short tile[kMaxMatrices + 1];   // [used + 1] first column tile
+    short column[kMaxRows];         // first column of each product, over all column tiles
+    short count[kMaxMatrices], place[kMaxMatrices];
     int used;
 };
 
 // Called by all threads of the block.
-template <int kThreads> __device__ void sort_products(Sorted& s, const int* matrix, int n, int E) {
+template <int kThreads, int kPlanes> __device__ void sort_products(Sorted& s, const int* matrix, int n, int E) {
     if (!matrix) {
-        for (int i = threadIdx.x; i < n; i += kThreads) s.rows[i] = (short)i;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            s.rows[i] = (short)i;
+            s.column[i] = (short)(i * kPlanes);
+        }
         if (threadIdx.x == 0) {
             s.used = 1;
-            s.matrix[0] = s.first[0] = 0;
+            s.matrix[0] = s.first[0] = s.tile[0] = 0;
             s.first[1] = (short)n;
+            s.tile[1] = (short)((n * kPlanes + 7) / 8);
         }
         __syncthreads();
         return;
@@ -191,28 +113,33 @@ template <int kThreads> __device__ void sort_products(Sorted& s, const int* matr
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-        int used = 0, at = 0;
+        int used = 0, at = 0, tiles = 0;
         for (int e0 = 0; e0 < E; e0 += 32) {
             const int e = e0 + threadIdx.x, c = e < E ? s.count[e] : 0;
-            int sum = c;
+            const int t = (c * kPlanes + 7) / 8;
+            int sum = c, tile = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, sum, o);
-                if (threadIdx.x >= o) sum += v;
+                const int v = __shfl_up_sync(0xffffffffu, sum, o), u = __shfl_up_sync(0xffffffffu, tile, o);
+                if (threadIdx.x >= o) sum += v, tile += u;
             }
             const unsigned m = __ballot_sync(0xffffffffu, c > 0);
             if (c > 0) {
                 const int k = used + __popc(m & ((1u << threadIdx.x) - 1));
                 s.matrix[k] = (short)e;
                 s.first[k] = (short)(at + sum - c);
+                s.tile[k] = (short)(tiles + tile - t);
+                s.place[e] = (short)k;
                 s.count[e] = (short)(at + sum - c);     // from here on the place of its first product
             }
             used += __popc(m);
             at += __shfl_sync(0xffffffffu, sum, 31);
+            tiles += __shfl_sync(0xffffffffu, tile, 31);
         }
         if (threadIdx.x == 0) {
             s.used = used;
             s.first[used] = (short)at;
+            s.tile[used] = (short)tiles;
         }
     }
     __syncthreads();
@@ -222,8 +149,114 @@ template <int kThreads> __device__ void sort_products(Sorted& s, const int* matr
         int rank = 0;
         for (int k = 0; k < i; ++k) rank += s.of[k] == e;
         s.rows[s.count[e] + rank] = (short)i;
+        s.column[i] = (short)(s.tile[s.place[e]] * 8 + rank * kPlanes);
     }
     __syncthreads();
+}
+
+// ------------------------------------------------------------ activations
+// The activations as the products' operand B: a row of x scaled by a power of
+// two to below 2^11, as one column (16-bit types: exact down to 2^-34 of the
+// row's largest) or two, hi and (x - hi) 2^11 (fp32: 22 bits).  The columns of
+// a matrix's products lie together, in tiles of 8, as the lanes hold them:
+//   plane   [column tile][block of 128][4 w][8 columns][4 j] 16 bytes: the
+//           float16 pairs (i, i + 4), i < 4, of inputs 32 w + 8 j .. + 7; with
+//           one plane those of even i times 16 to match their codes' 2^-24
+//   sums    [column tile][block of 128][128 / group][8 columns] of the scaled
+//           values, times 2^-20
+//   unit    [row of x] what a scaled sum is multiplied by
+struct Planes {
+    uint4* plane;
+    float* sums;
+    float* unit;
+};
+
+struct PlanesArgs {
+    const void* x;
+    long long stride;
+    const int* matrix;
+    Planes out;
+    int cols, blocks, group, num_rows, share, E;
+};
+
+// One block per row of x.
+template <class T, int kPlanes> __global__ void __launch_bounds__(512) w4_planes_kernel(PlanesArgs a) {
+    __shared__ float best[16];
+    __shared__ Sorted sorted;
+    const int row = blockIdx.x;
+    const T* p = static_cast<const T*>(a.x) + row * a.stride;
+    wait_predecessor_grid();
+    launch_dependents();
+    sort_products<512, kPlanes>(sorted, a.matrix, a.num_rows, a.E);
+    float mx = 0.0f;
+    for (int k = threadIdx.x; k < a.cols; k += 512) mx = fmaxf(mx, fabsf(to_f32(p[k])));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mx;
+    __syncthreads();
+    mx = best[threadIdx.x & 15];
+#pragma unroll
+    for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    // Exponent of the largest, kept where 2^(10 - e) is a normal number.
+    const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
+    const float up = __uint_as_float((264 - e) << 23);
+    if (threadIdx.x == 0) a.out.unit[row] = __uint_as_float((e - 10) << 23);
+    const int chunks = a.blocks * (kBlockK / 8), per = a.group / 8;
+    const int first = row * a.share, last = min(a.num_rows, first + a.share);
+    for (int c = threadIdx.x; c < chunks; c += 512) {    // chunks is a multiple of 16: whole groups of lanes
+        float v[8], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += v[i] = c * 8 < a.cols ? to_f32(p[c * 8 + i]) * up : 0.0f;
+        const unsigned live = __activemask();
+        for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = kPlanes == 2 || (i & 1) ? 1.0f : 16.0f;
+            const __half2 h = __floats2half2_rn(v[i] * f, v[i + 4] * f);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+            if constexpr (kPlanes == 2) {
+                const float2 b = __half22float2(h);
+                const __half2 l = __floats2half2_rn((v[i] * f - b.x) * 2048.0f, (v[i + 4] * f - b.y) * 2048.0f);
+                lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+            }
+        }
+        for (int i = first; i < last; ++i) {             // the products that share the row
+            if (a.matrix && sorted.of[i] < 0) continue;
+            const int column = sorted.column[i], block = c / 16;
+            const long long at = (long long)(column / 8) * a.blocks + block;
+            uint4* to = a.out.plane + at * 128 + c % 16 / 4 * 32 + column % 8 * 4 + c % 4;
+            to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (kPlanes == 2) to[4] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (kPlanes == 1 && c % per == 0)
+                a.out.sums[(at * (kBlockK / a.group) + c % 16 / per) * 8 + column % 8] = sum * (1.0f / 1048576.0f);
+        }
+    }
+}
+
+// --------------------------------------------------------------- products
+struct MatvecArgs {
+    const uint8_t* records;
+    Planes x;
+    const int* matrix;      // [num_rows], or null
+    void* y;                // [num_rows][outputs]
+    int num_rows, E, tiles, blocks, outputs, dtype;
+    FastDiv x_share, groups;   // groups: items of a matrix
+    bool gated;
+    int tiles_used;         // tiles with rows of the matrix
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ void store_as(void* y, long long at, float v, int dtype) {
+    if (dtype == MOE_DTYPE_F32) static_cast<float*>(y)[at] = v;
+    else if (dtype == MOE_DTYPE_BF16) static_cast<__nv_bfloat16*>(y)[at] = from_f32<__nv_bfloat16>(v);
+    else static_cast<__half*>(y)[at] = from_f32<__half>(v);
 }
 
 // y = W x.  An item is (matrix in use, MT tiles of 16 weight rows); the blocks
@@ -246,28 +279,30 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
     constexpr int kTokens = 8 * NT / kPlanes;                    // products per pass
     constexpr int kV = kPlanes == 2 ? 2 : 4;                     // sums per lane, tile and column tile
     constexpr int kDepth = 4 / MT, kUnroll = kDepth < 2 ? 2 : kDepth;
-    constexpr int kRecord = w4_record(kPer);
+    constexpr int kRecord = w4_record(kPer), kStep = 4 * kRecord * kWarps;   // from a warp's block of columns to its next
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     __shared__ float part[kWarps][MT * 16][kTokens + 1];
     __shared__ Sorted sorted;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-    sort_products<kThreads>(sorted, a.matrix, a.num_rows, a.E);
-    const int items = sorted.used * a.groups;
-    const long long tile_step = (long long)a.blocks * kRecord;
+    sort_products<kThreads, kPlanes>(sorted, a.matrix, a.num_rows, a.E);
+    const int items = sorted.used * a.groups.d;
 
     uint4 code[kDepth][MT][2];
     uint32_t par[kDepth][MT][2 * kPer];
     const uint8_t* base = nullptr;     // the item's records, at the lane's place
     auto begin = [&](int item) {
-        const int m = item / a.groups, tile = (item - m * a.groups) * MT;
-        base = a.records + ((long long)sorted.matrix[m] * a.tiles + tile) * tile_step + lane * 16;
+        const int m = a.groups.div(item), tile = (item - m * a.groups.d) * MT;
+        base = a.records + ((long long)sorted.matrix[m] * (a.tiles / 4) + tile / 4) * a.blocks * (4 * kRecord) +
+               (tile % 4) * kRecord + warp * (4 * kRecord);
     };
-    auto fetch = [&](int d, int t, int kb) {
-        if (kb < a.blocks) {
-            const uint8_t* rec = base + t * tile_step + (long long)kb * kRecord;
-            code[d][t][0] = load_stream(reinterpret_cast<const uint4*>(rec));
-            code[d][t][1] = load_stream(reinterpret_cast<const uint4*>(rec + 512));
-            const uint8_t* p = rec - lane * 16 + 1024 + g * (8 * kPer);
+    // Records of the warp's d-th block of columns from `at` on; the ring's place d.
+    const uint32_t code_at = lane * 16, par_at = 1024 + g * (8 * kPer);
+    auto fetch = [&](const uint8_t* at, int d, int t, bool live) {
+        if (live) {
+            const uint8_t* rec = at + t * kRecord;
+            code[d][t][0] = load_stream(reinterpret_cast<const uint4*>(rec + code_at));
+            code[d][t][1] = load_stream(reinterpret_cast<const uint4*>(rec + code_at + 512));
+            const uint8_t* p = rec + par_at;
             if constexpr (kPer == 1) {
                 const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
                 par[d][t][0] = v.x, par[d][t][1] = v.y;
@@ -284,7 +319,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
 #pragma unroll
         for (int d = 0; d < kDepth; ++d)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) fetch(d, t, warp + d * kWarps);
+            for (int t = 0; t < MT; ++t) fetch(base + d * kStep, d, t, warp + d * kWarps < a.blocks);
     };
     int item = blockIdx.x, t0 = 0;
     if (item < items) {
@@ -300,29 +335,26 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
     }
 
     while (item < items) {
-        const int m = item / a.groups, tile = (item - m * a.groups) * MT;
+        const int m = a.groups.div(item), tile = (item - m * a.groups.d) * MT;
         const short* rows = sorted.rows + sorted.first[m];
         const int n = sorted.first[m + 1] - sorted.first[m];
-        // The lane's column of B, and the rows whose sums it holds.
-        const uint4* bx[NT];
-        const float* sx[NT][2 / kPlanes];
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            auto x_row = [&](int token) { return rows[min(t0 + token, n - 1)] / a.x_share; };
-            const int col = c * 8 + g, token = col / kPlanes;
-            const long long per_row = (long long)a.blocks * 16;
-            bx[c] = t0 + token < n ? a.x.plane + (x_row(token) * kPlanes + col % kPlanes) * per_row + j : nullptr;
-#pragma unroll
-            for (int i = 0; i < 2 / kPlanes; ++i)
-                sx[c][i] = a.x.sums + (long long)x_row((c * 8 + 2 * j) / kPlanes + i) * a.blocks * kPer;
-        }
+        // The lane's part of B, and the sums of the columns whose products it
+        // holds; columns past the last product are not read, nor their sums.
+        const long long x_tile = sorted.tile[m] + t0 * kPlanes / 8;
+        const uint4* bx = a.x.plane + x_tile * a.blocks * 128 + lane;
+        const float* sx = a.x.sums + x_tile * a.blocks * (kPer * 8) + 2 * j;
+        const int x_step = a.blocks * 128, s_step = a.blocks * (kPer * 8);
+        const int live = (n - t0) * kPlanes - g;      // of the lane's columns c * 8 + g those below
         uint4 bw[2][NT][4];
         auto fetch_x = [&](uint4 (&b)[NT][4], int kb) {
+            if (kb < a.blocks) {
 #pragma unroll
-            for (int c = 0; c < NT; ++c)
+                for (int c = 0; c < NT; ++c)
+                    if (c * 8 < live) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    b[c][w] = bx[c] && kb < a.blocks ? __ldg(bx[c] + kb * 16 + w * 4) : make_uint4(0, 0, 0, 0);
+                        for (int w = 0; w < 4; ++w) b[c][w] = __ldg(bx + c * x_step + kb * 128 + w * 32);
+                    }
+            }
         };
         fetch_x(bw[0], warp);
         fetch_x(bw[1], warp + kWarps);
@@ -340,14 +372,16 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
             for (int d = 0; d < kUnroll; ++d) {
                 const int kb = kb0 + d * kWarps, slot = d % kDepth;
                 if (kb >= a.blocks) break;
+                const bool more = kb + kDepth * kWarps < a.blocks;
                 float sums[NT][2][kPer];
                 if constexpr (kPlanes == 1) {
 #pragma unroll
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int q = 0; q < kPer; ++q) sums[c][i][q] = __ldg(sx[c][i] + kb * kPer + q);
+                        for (int q = 0; q < kPer; ++q) {
+                            const float2 v = __ldg(reinterpret_cast<const float2*>(sx + c * s_step + (kb * kPer + q) * 8));
+                            sums[c][0][q] = v.x, sums[c][1][q] = v.y;
+                        }
                 }
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
@@ -397,16 +431,16 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
                                 } else {
 #pragma unroll
                                     for (int i = 0; i < 2; ++i) {
-                                        // acc is in units of 2^-20, the sums in ones.
-                                        const float v = fmaf(acc[c][2 * h + i], 1048576.0f, -p.y * sums[c][i][q]);
+                                        const float v = fmaf(-p.y, sums[c][i][q], acc[c][2 * h + i]);
                                         y[t][c][2 * h + i] = fmaf(p.x, v, y[t][c][2 * h + i]);
                                     }
                                 }
                             }
                         }
                     }
-                    fetch(slot, t, kb + kDepth * kWarps);
+                    fetch(base + kDepth * kStep, slot, t, more);
                 }
+                base += kStep;
                 fetch_x(bw[d % 2], kb + 2 * kWarps);
             }
         }
@@ -439,7 +473,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
         for (int i = threadIdx.x; i < out_rows * now; i += kThreads) {
             const int r = i % out_rows, token = i / out_rows;
             const int product = rows[t0 + token];
-            const float unit = __ldg(a.x.unit + product / a.x_share) * (kPlanes == 2 ? 1024.0f : 1.0f);
+            const float unit = __ldg(a.x.unit + a.x_share.div(product)) * (kPlanes == 2 ? 1024.0f : 1048576.0f);
             auto total = [&](int row) {
                 float v = 0.0f;
 #pragma unroll
@@ -509,8 +543,11 @@ void free_work(MoeW4* h) {
 int ensure_rows(MoeW4* h, int rows) {
     if (rows <= h->work_rows) return MOE_OK;
     free_work(h);   // waits for what still uses it
-    const size_t plane = (size_t)rows * 2 * h->blocks * 256, unit = rows * sizeof(float);
-    const size_t sums = (size_t)rows * h->blocks * (kBlockK / h->cfg.group) * sizeof(float);
+    // Column tiles: two columns a product, one not full for each matrix in use,
+    // and one that the last pass of a kernel of two column tiles may look at.
+    const size_t tiles = (size_t)(2 * rows + 7) / 8 + std::min(rows, h->cfg.num_matrices) + 1;
+    const size_t plane = tiles * h->blocks * 2048, unit = rows * sizeof(float);
+    const size_t sums = tiles * h->blocks * (kBlockK / h->cfg.group) * 8 * sizeof(float);
     const size_t result = (size_t)rows * h->outputs * sizeof(float);
     cudaError_t e = cudaMalloc(&h->x.plane, plane);
     if (e == cudaSuccess) e = cudaMalloc(&h->x.sums, sums);
@@ -605,8 +642,8 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
 
 template <int kPlanes, int MT, int NT>
 cudaError_t launch_product(const MoeW4* h, MatvecArgs a, int used, cudaStream_t s) {
-    a.groups = (a.tiles_used + MT - 1) / MT;
-    const dim3 grid((unsigned)std::min((long long)a.groups * used, (long long)h->sms * w4_blocks(NT))), block(w4_threads(NT));
+    a.groups = FastDiv((a.tiles_used + MT - 1) / MT);
+    const dim3 grid((unsigned)std::min((long long)a.groups.d * used, (long long)h->sms * w4_blocks(NT))), block(w4_threads(NT));
     switch (kBlockK / h->cfg.group) {
         case 1: return launch(w4_matvec_kernel<kPlanes, MT, NT, 1>, grid, block, 0, s, true, a);
         case 2: return launch(w4_matvec_kernel<kPlanes, MT, NT, 2>, grid, block, 0, s, true, a);
@@ -620,11 +657,11 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     const MoeW4Config& c = h->cfg;
     const int x_rows = (num_rows + x_share - 1) / x_share;
-    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 512, 0, s, dependent, x, (long long)x_stride, c.cols,
-                           h->blocks, c.group, h->x);
+    const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1};
+    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 512, 0, s, dependent, p);
     if (e != cudaSuccess) return e;
-    MatvecArgs a{h->records, h->x, matrix, y, num_rows, x_share, matrix ? c.num_matrices : 1, h->tiles, 0, h->blocks,
-                 h->outputs, dtype, c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
+    MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,
+                 FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
     // Columns of a matrix's products: all rows', or twice the mean's where the rows choose their matrices.
     const int columns = kPlanes * (matrix ? std::min(num_rows, 2 * ((num_rows + c.num_matrices - 1) / c.num_matrices)) : num_rows);
     const int used = matrix ? std::min(num_rows, c.num_matrices) : 1;
