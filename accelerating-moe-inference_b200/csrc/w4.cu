@@ -101,6 +101,44 @@ template <int kThreads, int kPlanes> __device__ void sort_products(Sorted& s, co
         __syncthreads();
         return;
     }
+    if (n <= 32) {       // one warp, a product a lane
+        if (threadIdx.x < 32) {
+            const int lane = threadIdx.x;
+            int e = lane < n ? __ldg(matrix + lane) : -1;
+            if (e >= E) e = -1;
+            const bool in = e >= 0;
+            const unsigned same = __match_any_sync(0xffffffffu, in ? e : -1), below = (1u << lane) - 1;
+            const int rank = __popc(same & below), count = __popc(same);
+            const bool leads = in && rank == 0;
+            int place = 0, first = 0, tile = 0, tiles_all = 0, all = 0;   // over the matrices before this one
+            for (int k = 0; k < n; ++k) {
+                const int other = __shfl_sync(0xffffffffu, leads ? e : -1, k), c = __shfl_sync(0xffffffffu, count, k);
+                const int t = (c * kPlanes + 7) / 8;
+                if (other < 0) continue;
+                all += c;
+                tiles_all += t;
+                if (other < e) ++place, first += c, tile += t;
+            }
+            const int used = __popc(__ballot_sync(0xffffffffu, leads));
+            if (lane < n) s.of[lane] = (short)(in ? e : -1);
+            if (in) {
+                s.rows[first + rank] = (short)lane;
+                s.column[lane] = (short)(tile * 8 + rank * kPlanes);
+            }
+            if (leads) {
+                s.matrix[place] = (short)e;
+                s.first[place] = (short)first;
+                s.tile[place] = (short)tile;
+            }
+            if (lane == 0) {
+                s.used = used;
+                s.first[used] = (short)all;
+                s.tile[used] = (short)tiles_all;
+            }
+        }
+        __syncthreads();
+        return;
+    }
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const int e = __ldg(matrix + i);
         s.of[i] = (short)(e >= 0 && e < E ? e : -1);
@@ -177,60 +215,124 @@ struct PlanesArgs {
     const int* matrix;
     Planes out;
     int cols, blocks, group, num_rows, share, E;
+    bool vec;              // rows of x can be read 16 bytes at a time
 };
 
-// One block per row of x.
-template <class T, int kPlanes> __global__ void __launch_bounds__(512) w4_planes_kernel(PlanesArgs a) {
-    __shared__ float best[16];
+// Eight inputs of a row from `k` on, zeros past its end.
+template <class T> __device__ __forceinline__ void load_chunk(const T* row, int k, int cols, bool vec, float (&v)[8]) {
+    if (k >= cols) {       // cols is a multiple of 32
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    } else if (vec) {
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8 * (int)sizeof(T) / 16; ++i)
+            *reinterpret_cast<uint4*>(t + i * (16 / sizeof(T))) = reinterpret_cast<const uint4*>(row + k)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(row[k + i]);
+    }
+}
+
+__device__ __forceinline__ float chunk_max(const float (&v)[8]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+    return m;
+}
+
+// Exponent of a row's largest, kept where 2^(10 - e) is a normal number, the
+// factor 2^(10 - e) that scales the row and its inverse.
+struct RowScale {
+    float up, unit;
+    __device__ explicit RowScale(float largest) {
+        const int e = min(max((int)(__float_as_uint(largest) >> 23), 11), 253);
+        up = __uint_as_float((264 - e) << 23);
+        unit = __uint_as_float((e - 10) << 23);
+    }
+};
+
+// A scaled chunk's operands.
+template <int kPlanes> __device__ __forceinline__ void operands(const float (&v)[8], uint4 (&out)[kPlanes]) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = kPlanes == 2 || (i & 1) ? 1.0f : 16.0f;
+        const __half2 h = __floats2half2_rn(v[i] * f, v[i + 4] * f);
+        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+        if constexpr (kPlanes == 2) {
+            const float2 b = __half22float2(h);
+            const __half2 l = __floats2half2_rn((v[i] - b.x) * 2048.0f, (v[i + 4] - b.y) * 2048.0f);
+            lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+    }
+    out[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if constexpr (kPlanes == 2) out[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// One block per row of x.  Latency is all: the row is read once, all its loads
+// at a time, and kept in registers (up to 16384 inputs; what is past them is
+// read again).
+template <class T, int kPlanes> __global__ void __launch_bounds__(1024) w4_planes_kernel(PlanesArgs a) {
+    constexpr int kHold = 2;
+    __shared__ float best[32];
     __shared__ Sorted sorted;
     const int row = blockIdx.x;
     const T* p = static_cast<const T*>(a.x) + row * a.stride;
     wait_predecessor_grid();
     launch_dependents();
-    sort_products<512, kPlanes>(sorted, a.matrix, a.num_rows, a.E);
-    float mx = 0.0f;
-    for (int k = threadIdx.x; k < a.cols; k += 512) mx = fmaxf(mx, fabsf(to_f32(p[k])));
+    const int chunks = a.blocks * (kBlockK / 8), per = a.group / 8;
+    float held[kHold][8], mx = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) load_chunk(p, (threadIdx.x + 1024 * h) * 8, a.cols, a.vec, held[h]);
+    sort_products<1024, kPlanes>(sorted, a.matrix, a.num_rows, a.E);
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) mx = fmaxf(mx, chunk_max(held[h]));
+    for (int c = threadIdx.x + 1024 * kHold; c < chunks; c += 1024) {
+        float v[8];
+        load_chunk(p, c * 8, a.cols, a.vec, v);
+        mx = fmaxf(mx, chunk_max(v));
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = mx;
     __syncthreads();
-    mx = best[threadIdx.x & 15];
+    mx = best[threadIdx.x & 31];
 #pragma unroll
-    for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    // Exponent of the largest, kept where 2^(10 - e) is a normal number.
-    const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
-    const float up = __uint_as_float((264 - e) << 23);
-    if (threadIdx.x == 0) a.out.unit[row] = __uint_as_float((e - 10) << 23);
-    const int chunks = a.blocks * (kBlockK / 8), per = a.group / 8;
+    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const RowScale scale(mx);
+    if (threadIdx.x == 0) a.out.unit[row] = scale.unit;
     const int first = row * a.share, last = min(a.num_rows, first + a.share);
-    for (int c = threadIdx.x; c < chunks; c += 512) {    // chunks is a multiple of 16: whole groups of lanes
-        float v[8], sum = 0.0f;
+    auto put = [&](int c, float (&v)[8]) {     // chunks is a multiple of 16: whole groups of lanes
+        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += v[i] = c * 8 < a.cols ? to_f32(p[c * 8 + i]) * up : 0.0f;
+        for (int i = 0; i < 8; ++i) sum += v[i] *= scale.up;
         const unsigned live = __activemask();
         for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float f = kPlanes == 2 || (i & 1) ? 1.0f : 16.0f;
-            const __half2 h = __floats2half2_rn(v[i] * f, v[i + 4] * f);
-            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-            if constexpr (kPlanes == 2) {
-                const float2 b = __half22float2(h);
-                const __half2 l = __floats2half2_rn((v[i] * f - b.x) * 2048.0f, (v[i + 4] * f - b.y) * 2048.0f);
-                lo[i] = *reinterpret_cast<const uint32_t*>(&l);
-            }
-        }
-        for (int i = first; i < last; ++i) {             // the products that share the row
+        uint4 b[kPlanes];
+        operands<kPlanes>(v, b);
+        for (int i = first; i < last; ++i) {   // the products that share the row
             if (a.matrix && sorted.of[i] < 0) continue;
             const int column = sorted.column[i], block = c / 16;
             const long long at = (long long)(column / 8) * a.blocks + block;
             uint4* to = a.out.plane + at * 128 + c % 16 / 4 * 32 + column % 8 * 4 + c % 4;
-            to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (kPlanes == 2) to[4] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int k = 0; k < kPlanes; ++k) to[4 * k] = b[k];
             if (kPlanes == 1 && c % per == 0)
                 a.out.sums[(at * (kBlockK / a.group) + c % 16 / per) * 8 + column % 8] = sum * (1.0f / 1048576.0f);
         }
+    };
+#pragma unroll
+    for (int h = 0; h < kHold; ++h) {
+        const int c = threadIdx.x + 1024 * h;
+        if (c < chunks) put(c, held[h]);
+    }
+    for (int c = threadIdx.x + 1024 * kHold; c < chunks; c += 1024) {
+        float v[8];
+        load_chunk(p, c * 8, a.cols, a.vec, v);
+        put(c, v);
     }
 }
 
@@ -657,8 +759,9 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     const MoeW4Config& c = h->cfg;
     const int x_rows = (num_rows + x_share - 1) / x_share;
-    const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1};
-    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 512, 0, s, dependent, p);
+    const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1,
+                       aligned16(x) && x_stride * (int64_t)sizeof(T) % 16 == 0};
+    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 1024, 0, s, dependent, p);
     if (e != cudaSuccess) return e;
     MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,
                  FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
