@@ -174,18 +174,46 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
 // ----------------------------------------------------------------- append
 // Eight consecutive elements as fp32; kVec: one or two 16-byte loads (the
 // address is 16-byte aligned), else element by element.
+__device__ __forceinline__ float2 pair_f32(uint32_t v, __nv_bfloat16) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ float2 pair_f32(uint32_t v, __half) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
 template <class T, bool kVec> __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-    if constexpr (kVec) {
-        constexpr int kN = 16 / sizeof(T);
-        T v[8];
+    if constexpr (kVec && sizeof(T) == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else if constexpr (kVec) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int i = 0; i < 8 / kN; ++i)
-            *reinterpret_cast<uint4*>(v + i * kN) = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_f32(w[i], T{});
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+    }
+}
+
+// The same as one or two 16-byte stores.
+__device__ __forceinline__ uint32_t pair_bits(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pair_bits(float a, float b, __half) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <class T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pair_bits(x[0], x[1], T{}), pair_bits(x[2], x[3], T{}),
+                                                  pair_bits(x[4], x[5], T{}), pair_bits(x[6], x[7], T{}));
     }
 }
 
@@ -198,72 +226,117 @@ struct AppendArgs {
     int N, H, bs, nb;
 };
 
-// One thread per 8 dims, 8 threads per group of 64, so a group's range is
-// three shuffles.  blockIdx.y: 0 keys, 1 values.
-template <class T, int D, bool kVec> __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
-    constexpr int G = D / 64, kThreads = D / 8;   // threads per (token, head)
-    const int kv = blockIdx.y;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long th = i / kThreads;            // token * H + head
-    const int m = (int)(i % kThreads);            // which 8 dims
-    const bool live = th < (long long)a.N * a.H;
-    const int token = live ? (int)(th / a.H) : 0, head = live ? (int)(th % a.H) : 0;
-    float x[8];
-    if (live) {
-        load8<T, kVec>(static_cast<const T*>(a.x[kv]) + token * a.token_stride[kv] + head * a.head_stride[kv] + m * 8, x);
-    } else {
+// Range of a group of 64 dims held by 8 neighbouring lanes, 8 dims each; the
+// lane's eight codes as a word, their scale and minimum, the values they stand for.
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& param) {
+    float lo = x[0], hi = x[0], sum = x[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    }
-    bool nan = false;
-    float lo = 65504.0f, hi = -65504.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        nan |= x[e] != x[e];
-        x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+    for (int e = 1; e < 8; ++e) {
         lo = fminf(lo, x[e]);
         hi = fmaxf(hi, x[e]);
+        sum += x[e];
+    }
+    // A NaN or an infinity shows in the sum, a value out of range in lo or hi.
+    unsigned nans = 0;
+    if (__any_sync(0xffffffffu, !(sum - sum == 0.0f) || lo < -65504.0f || hi > 65504.0f)) {
+        bool nan = false;
+        lo = 65504.0f, hi = -65504.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            nan |= x[e] != x[e];
+            x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+        nans = __ballot_sync(0xffffffffu, nan) >> ((threadIdx.x & 31) & ~7) & 0xff;
     }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    const unsigned nans = __ballot_sync(0xffffffffu, nan) >> ((threadIdx.x & 31) & ~7);
     __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), z = __float2half_rn(lo);
-    if (nans & 0xff) s = z = __ushort_as_half(0x7fff);
+    if (nans) s = z = __ushort_as_half(0x7fff);
+    param = __halves2half2(s, z);
     const float sf = __half2float(s), zf = __half2float(z);
+    // The quotient by the reciprocal, off by less than 1e-5; where that could
+    // change its rounding the division is done.  Adding 1.5 2^23 rounds to the
+    // nearest integer, ties to even, and leaves it in the sum's low bits.
+    constexpr float kRound = 12582912.0f;
+    const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
     uint32_t word = 0;
-    float val[8];
+    float c[8], far = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float q = sf > 0.0f ? rintf(__fdiv_rn(__fsub_rn(x[e], zf), sf)) : 0.0f;
-        const float c = fminf(fmaxf(q, 0.0f), 15.0f);
-        word |= (uint32_t)c << (4 * e);
-        val[e] = __fmaf_rn(sf, c, zf);   // s * c is exact in fp32
+        const float q = fminf(fmaxf((x[e] - zf) * inv, 0.0f), 15.0f);
+        const float t = __fadd_rn(q, kRound);
+        c[e] = __fsub_rn(t, kRound);
+        far = fmaxf(far, fabsf(q - c[e]));
+        word |= (__float_as_uint(t) & 15u) << (4 * e);
     }
-    if (!live) return;
-    if (a.out[kv]) {
-        T* o = static_cast<T*>(a.out[kv]) + th * D + m * 8;
-        T v[8];
+    if (far > 0.4999f) {
+        word = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(val[e]);
+        for (int e = 0; e < 8; ++e) {
+            c[e] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], zf), sf)), 0.0f), 15.0f);
+            word |= (uint32_t)c[e] << (4 * e);
+        }
+    }
 #pragma unroll
-        for (int e = 0; e < 8; e += 16 / (int)sizeof(T))
-            *reinterpret_cast<uint4*>(o + e) = *reinterpret_cast<const uint4*>(v + e);
+    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(sf, c[e], zf);   // s * c is exact in fp32
+    return word;
+}
+
+// A block quantises 16 tokens of one head, one thread per 8 dims of K and of V,
+// 8 threads per group of 64, so a group's range is three shuffles.  Bound by
+// reading k and v and writing the values back; a granule's codes lie in pieces
+// of 4 to 16 bytes per token, so 16 tokens that fill a granule (a prompt's, from
+// a multiple of 16 on) are put together in shared memory and written as whole
+// lines; others (a decode step's) are written piece by piece.
+template <class T, int D, bool kVec> __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
+    constexpr int G = D / 64, kThreads = 2 * D, kGran = kv4_granule(D);   // D / 8 threads per token
+    __shared__ __align__(16) uint8_t stage[kGran];
+    const int head = blockIdx.x % a.H, token0 = blockIdx.x / a.H * 16;
+    const int m = threadIdx.x % (D / 8), i = threadIdx.x / (D / 8), token = token0 + i, g = m >> 3;
+    const bool live = token < a.N;
+    float x[2][8];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        if (live) {
+            load8<T, kVec>(static_cast<const T*>(a.x[kv]) + token * a.token_stride[kv] + head * a.head_stride[kv] + m * 8, x[kv]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[kv][e] = 0.0f;
+        }
     }
-    const long long slot = a.slot[token];
-    if (slot < 0 || slot >= (long long)a.nb * a.bs) return;
-    const long long page = slot / a.bs;
-    const int off = (int)(slot % a.bs), t = off & 15, g = m >> 3;
-    uint8_t* gran = a.cache + ((page * a.H + head) * (a.bs >> 4) + (off >> 4)) * kv4_granule(D);
-    if (kv == 0) {
-        *reinterpret_cast<uint32_t*>(gran + kv4_k_word<D>(t, m)) = word;
-    } else {
-        *reinterpret_cast<uint32_t*>(gran + kv4_v_word<D>(t, m)) = word;
+    const long long slots = (long long)a.nb * a.bs, slot = live ? a.slot[token] : -1, slot0 = a.slot[token0];
+    const bool whole = __syncthreads_and(slot == slot0 + i && (slot0 & 15) == 0 && slot >= 0 && slot < slots);
+    const bool store = slot >= 0 && slot < slots;
+    const int t = (int)((whole ? i : slot) & 15);
+    uint8_t* gran = stage;
+    if (!whole && store) {
+        const long long page = slot / a.bs;
+        gran = a.cache + ((page * a.H + head) * (a.bs >> 4) + ((int)(slot % a.bs) >> 4)) * kGran;
     }
-    if ((m & 7) == 0)
-        *reinterpret_cast<__half2*>(gran + 16 * D + (kv * 16 + t) * G * 4 + g * 4) = __halves2half2(s, z);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        __half2 param;
+        const uint32_t word = quantise8(x[kv], param);
+        if (store) {
+            *reinterpret_cast<uint32_t*>(gran + (kv == 0 ? kv4_k_word<D>(t, m) : kv4_v_word<D>(t, m))) = word;
+            if ((m & 7) == 0) *reinterpret_cast<__half2*>(gran + 16 * D + (kv * 16 + t) * G * 4 + g * 4) = param;
+        }
+        if (live && a.out[kv]) {
+            T* o = static_cast<T*>(a.out[kv]) + ((long long)token * a.H + head) * D + m * 8;
+            store8(o, x[kv]);
+        }
+    }
+    if (whole) {
+        __syncthreads();
+        const long long page = slot0 / a.bs;
+        uint4* to = reinterpret_cast<uint4*>(a.cache + ((page * a.H + head) * (a.bs >> 4) + ((int)(slot0 % a.bs) >> 4)) * kGran);
+        for (int c = threadIdx.x; c < kGran / 16; c += kThreads) to[c] = reinterpret_cast<const uint4*>(stage)[c];
+    }
 }
 
 // -------------------------------------------------------------- attention
@@ -1116,7 +1189,9 @@ int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new
                    ring_state, block_table, kv_len, q_offset, position,
                    reinterpret_cast<long long*>(slot), ring_state_out};
         const size_t smem = (size_t)(2 * R + 1) * sizeof(int);
-        return launch_status(launch(plan_kernel, 1, kPlanThreads, smem, static_cast<cudaStream_t>(stream), false, a),
+        // As many blocks as there are threads' worth of tokens or warps' worth of requests, one per SM at most.
+        const int grid = std::max(1, std::min(h->sms, std::max(tokens_cap / kPlanThreads + 1, (R + 63) / 64)));
+        return launch_status(launch(plan_kernel, grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream), false, a),
                              "moe_kv4_plan_device");
     });
 }
@@ -1126,10 +1201,9 @@ int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new
 namespace {
 
 template <class T, int D> cudaError_t append_typed(const AppendArgs& a, bool vec, cudaStream_t s) {
-    const long long threads = (long long)a.N * a.H * (D / 8);
-    const dim3 grid((unsigned)((threads + 255) / 256), 2);
-    return vec ? launch(append_kernel<T, D, true>, grid, 256, 0, s, false, a)
-               : launch(append_kernel<T, D, false>, grid, 256, 0, s, false, a);
+    const dim3 grid((unsigned)((a.N + 15) / 16 * (long long)a.H));
+    return vec ? launch(append_kernel<T, D, true>, grid, 2 * D, 0, s, false, a)
+               : launch(append_kernel<T, D, false>, grid, 2 * D, 0, s, false, a);
 }
 
 template <class T> cudaError_t append_dim(const AppendArgs& a, int D, bool vec, cudaStream_t s) {
@@ -1161,7 +1235,7 @@ int moe_kv4_append_device(MoeKv4* h, void* cache, const void* k, const void* v, 
         const MoeKv4Config& c = h->cfg;
         if (!valid_dtype(dtype)) return report_error(MOE_ERR_INVALID, "moe_kv4_append_device: unknown dtype");
         if (tokens < 0) return report_error(MOE_ERR_INVALID, "moe_kv4_append_device: tokens must not be negative");
-        if ((long long)tokens * c.num_kv_heads * (c.head_dim / 8) > 0x7fffffffll * 128)
+        if (((long long)tokens + 15) / 16 * c.num_kv_heads > 0x7fffffffll)
             return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_append_device: too many tokens for one call");
         if (tokens == 0) return MOE_OK;
         if (!cache || !k || !v || !slot)
