@@ -14,33 +14,39 @@ namespace moe {
 namespace {
 
 // ------------------------------------------------------------------- plan
-// Sum of v over the threads before this one; *total the sum over all.  Every
-// thread of the block calls it; `buf` holds 33 values.
-__device__ long long block_scan(long long v, long long* buf, long long* total) {
+// Sums of v over the threads before this one; total the sums over all.  Every
+// thread of the block calls it; `buf` holds 33 pairs.
+struct Pair {
+    long long a, b;
+};
+__device__ __forceinline__ Pair shfl_up(Pair v, int o) {
+    return {__shfl_up_sync(0xffffffffu, v.a, o), __shfl_up_sync(0xffffffffu, v.b, o)};
+}
+__device__ Pair block_scan(Pair v, Pair* buf, Pair& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    long long inc = v;
+    Pair inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
+        const Pair u = shfl_up(inc, o);
+        if (lane >= o) inc.a += u.a, inc.b += u.b;
     }
     __syncthreads();
     if (lane == 31) buf[warp] = inc;
     __syncthreads();
     if (warp == 0) {
-        long long w = lane < warps ? buf[lane] : 0;
-        long long s = w;
+        const Pair w = lane < warps ? buf[lane] : Pair{0, 0};
+        Pair s = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += u;
+            const Pair u = shfl_up(s, o);
+            if (lane >= o) s.a += u.a, s.b += u.b;
         }
-        buf[lane] = s - w;
+        buf[lane] = {s.a - w.a, s.b - w.b};
         if (lane == 31) buf[32] = s;
     }
     __syncthreads();
-    *total = buf[32];
-    return buf[warp] + inc - v;
+    total = buf[32];
+    return {buf[warp].a + inc.a - v.a, buf[warp].b + inc.b - v.b};
 }
 
 struct PlanArgs {
@@ -55,6 +61,7 @@ struct PlanArgs {
     int* position;
     long long* slot;
     int* state_out;
+    FastDiv page;     // by bs
 };
 
 constexpr int kPlanThreads = 1024;
@@ -68,34 +75,34 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
     extern __shared__ int plan_smem[];
     int* q_off = plan_smem;              // [R + 1] clipped to cap
     int* first = plan_smem + a.R + 1;    // [R] first page taken from the ring; -1 rejected; or first page given back
-    __shared__ long long buf[33];
+    __shared__ Pair buf[33];
+    __shared__ int taken;
     const int per = (a.R + kPlanThreads - 1) / kPlanThreads;
     const int r0 = min(a.R, (int)threadIdx.x * per), r1 = min(a.R, r0 + per);
     int head = a.state[0], count = a.state[1];
     if (head < 0 || head >= a.nb || count < 0 || count > a.nb) head = count = 0;
     const long long limit = (long long)a.W * a.bs;
 
-    long long grow = 0, total;
-    for (int r = r0; r < r1; ++r) grow += max(0, a.added[r]);
-    const long long begin = block_scan(grow, buf, &total);
-    const long long tokens = total;
+    if (threadIdx.x == 0) taken = 0;
+    // Positions count within pages: 0 <= n <= W * bs <= 2^30.
+    auto pages = [&](long long n) { return a.page.div((int)n + a.bs - 1); };
+    Pair total, sum{0, 0};
+    for (int r = r0; r < r1; ++r) sum.a += max(0, a.added[r]);
+    const long long begin = block_scan(sum, buf, total).a, tokens = total.a;
     long long end = begin;
-    long long need = 0, back = 0;
+    sum = {0, 0};   // pages needed, pages given back
     for (int r = r0; r < r1; ++r) {
         const long long c = a.cached[r], n = a.added[r];
         q_off[r] = (int)min(end, (long long)a.cap);
         end += max(0ll, n);
         if (c < 0 || c > limit) continue;
-        if (n >= 0 && c + n <= limit && (n == 0 || end <= a.cap)) need += (c + n + a.bs - 1) / a.bs - (c + a.bs - 1) / a.bs;
-        if (n < 0) back += (c + a.bs - 1) / a.bs;
+        if (n >= 0 && c + n <= limit && (n == 0 || end <= a.cap)) sum.a += pages(c + n) - pages(c);
+        if (n < 0) sum.b += pages(c);
     }
     if (threadIdx.x == 0) q_off[a.R] = (int)min(tokens, (long long)a.cap);
-    long long all;
-    long long nsum = block_scan(need, buf, &all);
-    long long bsum = block_scan(back, buf, &total);
-    const long long given = min(total, (long long)a.nb - count);
+    Pair before = block_scan(sum, buf, total);
+    const long long given = min(total.b, (long long)a.nb - count);
     end = begin;
-    long long taken = 0;
     for (int r = r0; r < r1; ++r) {
         const long long c = a.cached[r], n = a.added[r];
         end += max(0ll, n);
@@ -104,16 +111,17 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
         first[r] = -1;
         if (c >= 0 && c <= limit) {
             if (n >= 0 && c + n <= limit && (n == 0 || end <= a.cap)) {
-                take = (c + n + a.bs - 1) / a.bs - (c + a.bs - 1) / a.bs;
-                ok = take == 0 || nsum + take <= count;
+                take = pages(c + n) - pages(c);
+                ok = take == 0 || before.a + take <= count;
                 if (ok) {
-                    first[r] = (int)min(nsum, (long long)count);
-                    taken += take;
+                    first[r] = (int)min(before.a, (long long)count);
+                    // The needs of the admitted are a prefix of all needs.
+                    if (take) atomicMax(&taken, (int)(before.a + take));
                 }
-                nsum += take;
+                before.a += take;
             } else if (n < 0) {
-                first[r] = (int)min(bsum, given);
-                bsum += (c + a.bs - 1) / a.bs;
+                first[r] = (int)min(before.b, given);
+                before.b += pages(c);
             }
         }
         if (blockIdx.x == 0) {
@@ -121,29 +129,42 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
             a.q_offset[r] = q_off[r];
         }
     }
-    block_scan(taken, buf, &total);
+    __syncthreads();
+    // Places in the ring are below 2 nb: head < nb, and count plus what is
+    // given back is at most nb.
+    auto wrap = [&](long long i) { return (int)(i >= a.nb ? i - a.nb : i); };
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         a.q_offset[a.R] = q_off[a.R];
-        a.state_out[0] = (int)((head + total) % a.nb);
-        a.state_out[1] = (int)(count - total + given);
+        a.state_out[0] = wrap((long long)head + taken);
+        a.state_out[1] = (int)(count - taken + given);
     }
-    __syncthreads();
 
-    // The requests' rows: a warp each.
+    // The requests' rows: a warp each, 256 pages' loads in flight.
     const int lane = threadIdx.x & 31;
+    auto copy = [&](int n, auto from, auto to) {
+        for (int i0 = lane; i0 < n; i0 += 256) {
+            int v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + 32 * k < n) v[k] = from(i0 + 32 * k);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i0 + 32 * k < n) to(i0 + 32 * k, v[k]);
+        }
+    };
     const int warps = gridDim.x * (kPlanThreads / 32);
     for (int r = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5); r < a.R; r += warps) {
         const int f = first[r];
         if (f < 0) continue;
         const long long c = a.cached[r], n = a.added[r];
-        const long long used = (c + a.bs - 1) / a.bs;
+        const int used = pages(c);
         int* row = a.table + (size_t)r * a.W;
         if (n < 0) {
-            for (long long i = lane; i < used && f + i < given; i += 32)
-                a.ring[((long long)head + count + f + i) % a.nb] = row[i];
+            copy((int)min((long long)used, given - f), [&](int i) { return row[i]; },
+                 [&](int i, int v) { a.ring[wrap((long long)head + count + f + i)] = v; });
         } else {
-            const long long take = (c + n + a.bs - 1) / a.bs - used;
-            for (long long i = lane; i < take; i += 32) row[used + i] = a.ring[((long long)head + f + i) % a.nb];
+            const int take = pages(c + n) - used;
+            copy(take, [&](int i) { return a.ring[wrap((long long)head + f + i)]; }, [&](int i, int v) { row[used + i] = v; });
         }
     }
     // The tokens: a thread each.
@@ -160,10 +181,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
             const int c = a.cached[lo];
             pos = (int)((unsigned)c + (unsigned)(t - q_off[lo]));   // out of range only where rejected
             if (first[lo] >= 0) {
-                const int used = (int)(((long long)c + a.bs - 1) / a.bs), b = pos / a.bs;
+                const int used = pages(c), b = a.page.div(pos);
                 const int page = b < used ? a.table[(size_t)lo * a.W + b]
-                                          : a.ring[((long long)head + first[lo] + b - used) % a.nb];
-                if (page >= 0 && page < a.nb) slot = (long long)page * a.bs + pos % a.bs;
+                                          : a.ring[wrap((long long)head + first[lo] + b - used)];
+                if (page >= 0 && page < a.nb) slot = (long long)page * a.bs + pos - b * a.bs;
             }
         }
         a.position[t] = pos;
@@ -224,6 +245,8 @@ struct AppendArgs {
     const long long* slot;
     void* out[2];
     int N, H, bs, nb;
+    FastDiv heads;    // by H
+    FastDiv page;     // by bs / 16
 };
 
 // Range of a group of 64 dims held by 8 neighbouring lanes, 8 dims each; the
@@ -296,7 +319,7 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& param) {
 template <class T, int D, bool kVec> __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
     constexpr int G = D / 64, kThreads = 2 * D, kGran = kv4_granule(D);   // D / 8 threads per token
     __shared__ __align__(16) uint8_t stage[kGran];
-    const int head = blockIdx.x % a.H, token0 = blockIdx.x / a.H * 16;
+    const int group = a.heads.div(blockIdx.x), head = blockIdx.x - group * a.H, token0 = group * 16;
     const int m = threadIdx.x % (D / 8), i = threadIdx.x / (D / 8), token = token0 + i, g = m >> 3;
     const bool live = token < a.N;
     float x[2][8];
@@ -313,11 +336,11 @@ template <class T, int D, bool kVec> __global__ void __launch_bounds__(2 * D) ap
     const bool whole = __syncthreads_and(slot == slot0 + i && (slot0 & 15) == 0 && slot >= 0 && slot < slots);
     const bool store = slot >= 0 && slot < slots;
     const int t = (int)((whole ? i : slot) & 15);
-    uint8_t* gran = stage;
-    if (!whole && store) {
-        const long long page = slot / a.bs;
-        gran = a.cache + ((page * a.H + head) * (a.bs >> 4) + ((int)(slot % a.bs) >> 4)) * kGran;
-    }
+    auto granule = [&](long long at) {     // of a slot: at / 16 is below 2^31
+        const int n = (int)(at >> 4), page = a.page.div(n);
+        return a.cache + (((long long)page * a.H + head) * a.page.d + n - page * a.page.d) * kGran;
+    };
+    uint8_t* gran = !whole && store ? granule(slot) : stage;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
         __half2 param;
@@ -333,8 +356,7 @@ template <class T, int D, bool kVec> __global__ void __launch_bounds__(2 * D) ap
     }
     if (whole) {
         __syncthreads();
-        const long long page = slot0 / a.bs;
-        uint4* to = reinterpret_cast<uint4*>(a.cache + ((page * a.H + head) * (a.bs >> 4) + ((int)(slot0 % a.bs) >> 4)) * kGran);
+        uint4* to = reinterpret_cast<uint4*>(granule(slot0));
         for (int c = threadIdx.x; c < kGran / 16; c += kThreads) to[c] = reinterpret_cast<const uint4*>(stage)[c];
     }
 }
@@ -505,7 +527,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     constexpr int kStage = 2 * kGran;
     constexpr int kWarpFloats = kRows * kPitch + 2 * kRows;   // a warp's result
     extern __shared__ __align__(16) uint8_t attend_smem[];
-    __shared__ long long scan_buf[33];
+    __shared__ Pair scan_buf[33];
     __shared__ long long start_unit;
     __shared__ int start_r, is_last, join_from, join_to;
     __shared__ Walk ahead_walk[kAttendWarps];
@@ -520,9 +542,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     // The block's share of the units, and the request its first one lies in.
     const int per = (a.R + kThreads - 1) / kThreads;
     const int r0 = min(a.R, (int)threadIdx.x * per), r1 = min(a.R, r0 + per);
-    long long mine = 0, total;
+    long long mine = 0;
     for (int r = r0; r < r1; ++r) mine += request_of<kRows>(a, r).units;
-    long long base = block_scan(mine, scan_buf, &total);
+    Pair sums;
+    long long base = block_scan({mine, 0}, scan_buf, sums).a;
+    const long long total = sums.a;
     const long long chunk = max((total + gridDim.x - 1) / gridDim.x, (long long)kAttendMinUnits);
     const long long u0 = blockIdx.x * chunk;
     if (u0 >= total) return;
@@ -1105,8 +1129,9 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
             return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_create: head_dim must be 64 or 128");
         if (cfg->block_tokens < 16 || cfg->block_tokens > 1024 || cfg->block_tokens % 16)
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: block_tokens must be a multiple of 16, 16..1024");
-        if ((long long)cfg->num_blocks * cfg->num_kv_heads * (cfg->block_tokens / 16) >= 0xffffffffll)
-            return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_create: a cache of 2^32 granules or more");
+        if ((long long)cfg->num_blocks * cfg->num_kv_heads * (cfg->block_tokens / 16) >= 0xffffffffll ||
+            (long long)cfg->num_blocks * (cfg->block_tokens / 16) > 0x7fffffffll)
+            return report_error(MOE_ERR_UNSUPPORTED, "moe_kv4_create: a cache of 2^32 granules, or of 2^31 per head, or more");
         if (cfg->num_blocks < 1 || cfg->table_width < 1 ||
             (long long)cfg->table_width * cfg->block_tokens > (1 << 30))
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: need num_blocks >= 1, table_width >= 1 and "
@@ -1187,7 +1212,7 @@ int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_plan_device: cannot select the device");
         PlanArgs a{cached_len, new_len, R, c.table_width, c.block_tokens, c.num_blocks, tokens_cap, free_ring,
                    ring_state, block_table, kv_len, q_offset, position,
-                   reinterpret_cast<long long*>(slot), ring_state_out};
+                   reinterpret_cast<long long*>(slot), ring_state_out, FastDiv(c.block_tokens)};
         const size_t smem = (size_t)(2 * R + 1) * sizeof(int);
         // As many blocks as there are threads' worth of tokens or warps' worth of requests, one per SM at most.
         const int grid = std::max(1, std::min(h->sms, std::max(tokens_cap / kPlanThreads + 1, (R + 63) / 64)));
@@ -1249,7 +1274,7 @@ int moe_kv4_append_device(MoeKv4* h, void* cache, const void* k, const void* v, 
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_append_device: cannot select the device");
         AppendArgs a{static_cast<uint8_t*>(cache), {k, v}, {k_token_stride, v_token_stride},
                      {k_head_stride, v_head_stride}, reinterpret_cast<const long long*>(slot), {k_out, v_out}, tokens,
-                     c.num_kv_heads, c.block_tokens, c.num_blocks};
+                     c.num_kv_heads, c.block_tokens, c.num_blocks, FastDiv(c.num_kv_heads), FastDiv(c.block_tokens / 16)};
         bool vec = aligned16(k) && aligned16(v);
         for (int64_t st : {k_token_stride, k_head_stride, v_token_stride, v_head_stride})
             vec = vec && (st * (int64_t)es) % 16 == 0;
