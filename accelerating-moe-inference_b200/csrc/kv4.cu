@@ -251,25 +251,28 @@ struct AppendArgs {
 
 // Range of a group of 64 dims held by 8 neighbouring lanes, 8 dims each; the
 // lane's eight codes as a word, their scale and minimum, the values they stand for.
-__device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& param) {
-    float lo = x[0], hi = x[0], sum = x[0];
+__device__ __forceinline__ uint32_t quantise8(float2 (&x)[4], __half2& param) {
+    float lo = fminf(x[0].x, x[0].y), hi = fmaxf(x[0].x, x[0].y);
+    float2 sum = x[0];
 #pragma unroll
-    for (int e = 1; e < 8; ++e) {
-        lo = fminf(lo, x[e]);
-        hi = fmaxf(hi, x[e]);
-        sum += x[e];
+    for (int e = 1; e < 4; ++e) {
+        lo = fminf(lo, fminf(x[e].x, x[e].y));
+        hi = fmaxf(hi, fmaxf(x[e].x, x[e].y));
+        sum = __fadd2_rn(sum, x[e]);
     }
     // A NaN or an infinity shows in the sum, a value out of range in lo or hi.
     unsigned nans = 0;
-    if (__any_sync(0xffffffffu, !(sum - sum == 0.0f) || lo < -65504.0f || hi > 65504.0f)) {
+    const float all = sum.x + sum.y;
+    if (__any_sync(0xffffffffu, !(all - all == 0.0f) || lo < -65504.0f || hi > 65504.0f)) {
         bool nan = false;
         lo = 65504.0f, hi = -65504.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            nan |= x[e] != x[e];
-            x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
+        for (int e = 0; e < 4; ++e) {
+            nan |= x[e].x != x[e].x || x[e].y != x[e].y;
+            x[e].x = fminf(fmaxf(x[e].x, -65504.0f), 65504.0f);
+            x[e].y = fminf(fmaxf(x[e].y, -65504.0f), 65504.0f);
+            lo = fminf(lo, fminf(x[e].x, x[e].y));
+            hi = fmaxf(hi, fmaxf(x[e].x, x[e].y));
         }
         nans = __ballot_sync(0xffffffffu, nan) >> ((threadIdx.x & 31) & ~7) & 0xff;
     }
@@ -287,71 +290,97 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], __half2& param) {
     // nearest integer, ties to even, and leaves it in the sum's low bits.
     constexpr float kRound = 12582912.0f;
     const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
+    const float2 down = make_float2(-zf, -zf), by = make_float2(inv, inv), round = make_float2(kRound, kRound),
+                 back = make_float2(-kRound, -kRound);
     uint32_t word = 0;
-    float c[8], far = 0.0f;
+    float2 c[4];
+    float far = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float q = fminf(fmaxf((x[e] - zf) * inv, 0.0f), 15.0f);
-        const float t = __fadd_rn(q, kRound);
-        c[e] = __fsub_rn(t, kRound);
-        far = fmaxf(far, fabsf(q - c[e]));
-        word |= (__float_as_uint(t) & 15u) << (4 * e);
+    for (int e = 0; e < 4; ++e) {
+        float2 q = __fmul2_rn(__fadd2_rn(x[e], down), by);
+        q.x = fminf(fmaxf(q.x, 0.0f), 15.0f);
+        q.y = fminf(fmaxf(q.y, 0.0f), 15.0f);
+        const float2 t = __fadd2_rn(q, round);
+        c[e] = __fadd2_rn(t, back);
+        const float2 off = __ffma2_rn(c[e], make_float2(-1.0f, -1.0f), q);
+        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+        const uint32_t two = __float_as_uint(t.x) & 15u | __float_as_uint(t.y) << 4;   // above 8 bits: kRound's
+        word |= (two & 255u) << (8 * e);
     }
     if (far > 0.4999f) {
         word = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            c[e] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e], zf), sf)), 0.0f), 15.0f);
-            word |= (uint32_t)c[e] << (4 * e);
+        for (int e = 0; e < 4; ++e) {
+            c[e].x = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e].x, zf), sf)), 0.0f), 15.0f);
+            c[e].y = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[e].y, zf), sf)), 0.0f), 15.0f);
+            word |= ((uint32_t)c[e].x | (uint32_t)c[e].y << 4) << (8 * e);
         }
     }
+    const float2 scale = make_float2(sf, sf), zero = make_float2(zf, zf);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn(sf, c[e], zf);   // s * c is exact in fp32
+    for (int e = 0; e < 4; ++e) x[e] = __ffma2_rn(scale, c[e], zero);   // s * c is exact in fp32
     return word;
 }
 
-// A block quantises 16 tokens of one head, one thread per 8 dims of K and of V,
-// 8 threads per group of 64, so a group's range is three shuffles.  Bound by
-// reading k and v and writing the values back; a granule's codes lie in pieces
-// of 4 to 16 bytes per token, so 16 tokens that fill a granule (a prompt's, from
-// a multiple of 16 on) are put together in shared memory and written as whole
-// lines; others (a decode step's) are written piece by piece.
-template <class T, int D, bool kVec> __global__ void __launch_bounds__(2 * D) append_kernel(AppendArgs a) {
-    constexpr int G = D / 64, kThreads = 2 * D, kGran = kv4_granule(D);   // D / 8 threads per token
+// A block quantises 16 tokens of one head, a thread 8 dims of K and of V of
+// tokens i and i + 8; 8 threads hold a group of 64, so its range is three
+// shuffles.  A granule's codes lie in pieces of 4 to 16 bytes per token, so 16
+// tokens that fill a granule (a prompt's, from a multiple of 16 on) are put
+// together in shared memory and written as whole lines; others (a decode
+// step's) are written piece by piece.  Bound by its instructions, about 25 a
+// value, most of them the quantiser's, hence the pairwise fp32 operations.
+template <class T, int D, bool kVec> __global__ void __launch_bounds__(D, 1024 / D) append_kernel(AppendArgs a) {
+    constexpr int G = D / 64, kThreads = D, kGran = kv4_granule(D);   // D / 8 threads per token
     __shared__ __align__(16) uint8_t stage[kGran];
     const int group = a.heads.div(blockIdx.x), head = blockIdx.x - group * a.H, token0 = group * 16;
-    const int m = threadIdx.x % (D / 8), i = threadIdx.x / (D / 8), token = token0 + i, g = m >> 3;
-    const bool live = token < a.N;
-    float x[2][8];
+    const int m = threadIdx.x % (D / 8), i = threadIdx.x / (D / 8), g = m >> 3;
+    float2 x[2][2][4];      // [token][K, V]
+    const long long slots = (long long)a.nb * a.bs, slot0 = a.slot[token0];
+    long long slot[2];
+    bool fits = (slot0 & 15) == 0 && slot0 >= 0 && slot0 < slots;
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        if (live) {
-            load8<T, kVec>(static_cast<const T*>(a.x[kv]) + token * a.token_stride[kv] + head * a.head_stride[kv] + m * 8, x[kv]);
-        } else {
+    for (int h = 0; h < 2; ++h) {
+        const int token = token0 + i + 8 * h;
+        const bool live = token < a.N;
+        slot[h] = live ? a.slot[token] : -1;
+        fits = fits && slot[h] == slot0 + i + 8 * h;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[kv][e] = 0.0f;
+        for (int kv = 0; kv < 2; ++kv) {
+            if (live) {
+                float v[8];
+                load8<T, kVec>(static_cast<const T*>(a.x[kv]) + token * a.token_stride[kv] + head * a.head_stride[kv] + m * 8, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[h][kv][e] = make_float2(v[2 * e], v[2 * e + 1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[h][kv][e] = make_float2(0.0f, 0.0f);
+            }
         }
     }
-    const long long slots = (long long)a.nb * a.bs, slot = live ? a.slot[token] : -1, slot0 = a.slot[token0];
-    const bool whole = __syncthreads_and(slot == slot0 + i && (slot0 & 15) == 0 && slot >= 0 && slot < slots);
-    const bool store = slot >= 0 && slot < slots;
-    const int t = (int)((whole ? i : slot) & 15);
+    const bool whole = __syncthreads_and(fits);
     auto granule = [&](long long at) {     // of a slot: at / 16 is below 2^31
         const int n = (int)(at >> 4), page = a.page.div(n);
         return a.cache + (((long long)page * a.H + head) * a.page.d + n - page * a.page.d) * kGran;
     };
-    uint8_t* gran = !whole && store ? granule(slot) : stage;
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        __half2 param;
-        const uint32_t word = quantise8(x[kv], param);
-        if (store) {
-            *reinterpret_cast<uint32_t*>(gran + (kv == 0 ? kv4_k_word<D>(t, m) : kv4_v_word<D>(t, m))) = word;
-            if ((m & 7) == 0) *reinterpret_cast<__half2*>(gran + 16 * D + (kv * 16 + t) * G * 4 + g * 4) = param;
-        }
-        if (live && a.out[kv]) {
-            T* o = static_cast<T*>(a.out[kv]) + ((long long)token * a.H + head) * D + m * 8;
-            store8(o, x[kv]);
+    for (int h = 0; h < 2; ++h) {
+        const int token = token0 + i + 8 * h;
+        const bool store = slot[h] >= 0 && slot[h] < slots;
+        const int t = whole ? i + 8 * h : (int)(slot[h] & 15);
+        uint8_t* gran = !whole && store ? granule(slot[h]) : stage;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            __half2 param;
+            const uint32_t word = quantise8(x[h][kv], param);
+            if (store) {
+                *reinterpret_cast<uint32_t*>(gran + (kv == 0 ? kv4_k_word<D>(t, m) : kv4_v_word<D>(t, m))) = word;
+                if ((m & 7) == 0) *reinterpret_cast<__half2*>(gran + 16 * D + (kv * 16 + t) * G * 4 + g * 4) = param;
+            }
+            if (a.out[kv] && token < a.N) {
+                const float v[8] = {x[h][kv][0].x, x[h][kv][0].y, x[h][kv][1].x, x[h][kv][1].y,
+                                    x[h][kv][2].x, x[h][kv][2].y, x[h][kv][3].x, x[h][kv][3].y};
+                store8(static_cast<T*>(a.out[kv]) + ((long long)token * a.H + head) * D + m * 8, v);
+            }
         }
     }
     if (whole) {
@@ -1227,8 +1256,8 @@ namespace {
 
 template <class T, int D> cudaError_t append_typed(const AppendArgs& a, bool vec, cudaStream_t s) {
     const dim3 grid((unsigned)((a.N + 15) / 16 * (long long)a.H));
-    return vec ? launch(append_kernel<T, D, true>, grid, 2 * D, 0, s, false, a)
-               : launch(append_kernel<T, D, false>, grid, 2 * D, 0, s, false, a);
+    return vec ? launch(append_kernel<T, D, true>, grid, D, 0, s, false, a)
+               : launch(append_kernel<T, D, false>, grid, D, 0, s, false, a);
 }
 
 template <class T> cudaError_t append_dim(const AppendArgs& a, int D, bool vec, cudaStream_t s) {
