@@ -2,6 +2,7 @@
 // experts built on them.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 #include <new>
 
 #include "dtype.cuh"
@@ -15,6 +16,7 @@ namespace {
 constexpr int kMaxRows = 512;        // products of one call
 constexpr int kBlockK = 128;         // columns of a record
 constexpr int kMaxMatrices = 256;
+constexpr int kInlineMax = 49152;    // bytes of operands that a block makes for itself
 // Threads of a block and blocks of an SM, by column tiles: registers.
 __host__ __device__ constexpr int w4_threads(int NT) { return NT == 1 ? 256 : 128; }
 __host__ __device__ constexpr int w4_blocks(int NT) { return NT == 1 ? 2 : 3; }
@@ -375,8 +377,14 @@ __device__ __forceinline__ void store_as(void* y, long long at, float v, int dty
 // with two (fp32), where the sum's last bits count, code and zero become the
 // normal number (c - z) 2^-10 by one fma.  The warps' sums are added in order
 // through shared memory.
-template <int kPlanes, int MT, int NT, int kPer>
-__global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kernel(MatvecArgs a) {
+//
+// kInline: few activations (product() below) are made operands by every block for
+// itself, in shared memory, instead of by a kernel of their own; that saves a
+// launch where launches are what a product costs.
+template <class T, int MT, int NT, int kPer, bool kInline>
+__global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kernel(MatvecArgs a, PlanesArgs xa) {
+    static_assert(!kInline || NT == 1, "inline operands have one column tile");
+    constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     constexpr int kThreads = w4_threads(NT), kWarps = kThreads / 32;
     constexpr int kTokens = 8 * NT / kPlanes;                    // products per pass
     constexpr int kV = kPlanes == 2 ? 2 : 4;                     // sums per lane, tile and column tile
@@ -385,6 +393,9 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     __shared__ float part[kWarps][MT * 16][kTokens + 1];
     __shared__ Sorted sorted;
+    __shared__ float units[8];
+    __shared__ int largest[8];
+    extern __shared__ __align__(16) uint4 inline_x[];   // [block * 4 + w][column][4 j], then the sums
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
     sort_products<kThreads, kPlanes>(sorted, a.matrix, a.num_rows, a.E);
     const int items = sorted.used * a.groups.d;
@@ -436,16 +447,79 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
                 for (int r = lane; r < a.outputs; r += 32) store_as(a.y, (long long)i * a.outputs + r, 0.0f, a.dtype);
     }
 
+    // The operands of `tokens` products from `rows` on, at most 8 columns.
+    int made_m = -1, made_t0 = -1, made_row = -1;
+    auto make_x = [&](const short* rows, int tokens) {
+        const int columns = tokens * kPlanes, chunks = a.blocks * (kBlockK / 8);
+        constexpr int kChunks = kBlockK / kPer / 8;      // of a group
+        float* sums = reinterpret_cast<float*>(inline_x + a.blocks * 16 * columns);
+        __syncthreads();
+        if (threadIdx.x < tokens) largest[threadIdx.x] = 0;
+        __syncthreads();
+        auto row_of = [&](int t) { return static_cast<const T*>(xa.x) + a.x_share.div(rows[t]) * xa.stride; };
+        for (int t = 0; t < tokens; ++t) {
+            const T* p = row_of(t);
+            float mx = 0.0f;
+            for (int c = threadIdx.x; c < chunks; c += kThreads) {
+                float v[8];
+                load_chunk(p, c * 8, xa.cols, xa.vec, v);
+                mx = fmaxf(mx, chunk_max(v));
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if (lane == 0) atomicMax(largest + t, __float_as_int(mx));   // not negative: ordered as integers
+        }
+        __syncthreads();
+        for (int t = 0; t < tokens; ++t) {
+            const T* p = row_of(t);
+            const RowScale scale(__int_as_float(largest[t]));
+            if (threadIdx.x == 0) units[t] = scale.unit;
+            for (int c = threadIdx.x; c < chunks; c += kThreads) {       // whole groups of lanes
+                float v[8], sum = 0.0f;
+                load_chunk(p, c * 8, xa.cols, xa.vec, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += v[i] *= scale.up;
+                uint4 b[kPlanes];
+                operands<kPlanes>(v, b);
+#pragma unroll
+                for (int k = 0; k < kPlanes; ++k) inline_x[(c / 4 * columns + t * kPlanes + k) * 4 + c % 4] = b[k];
+                if constexpr (kPlanes == 1) {
+                    const unsigned live = __activemask();
+#pragma unroll
+                    for (int o = 1; o < kChunks; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
+                    if (c % kChunks == 0) sums[c / kChunks * 8 + t] = sum * (1.0f / 1048576.0f);
+                }
+            }
+        }
+        __syncthreads();
+    };
+
     while (item < items) {
         const int m = a.groups.div(item), tile = (item - m * a.groups.d) * MT;
         const short* rows = sorted.rows + sorted.first[m];
         const int n = sorted.first[m + 1] - sorted.first[m];
         // The lane's part of B, and the sums of the columns whose products it
         // holds; columns past the last product are not read, nor their sums.
-        const long long x_tile = sorted.tile[m] + t0 * kPlanes / 8;
-        const uint4* bx = a.x.plane + x_tile * a.blocks * 128 + lane;
-        const float* sx = a.x.sums + x_tile * a.blocks * (kPer * 8) + 2 * j;
-        const int x_step = a.blocks * 128, s_step = a.blocks * (kPer * 8);
+        const int columns = min(kTokens, n - t0) * kPlanes;
+        const uint4* bx;
+        const float* sx;
+        int x_block, x_word, x_step = 0, s_step = 0;   // from block to block, word to word, column tile to column tile
+        if constexpr (kInline) {
+            const int row = a.x_share.div(rows[t0]);
+            // One product's row may serve several matrices.
+            if (!(made_m == m && made_t0 == t0) && !(columns == kPlanes && made_row == row)) make_x(rows + t0, columns / kPlanes);
+            made_m = m, made_t0 = t0, made_row = columns == kPlanes ? row : -1;
+            bx = inline_x + lane;
+            sx = reinterpret_cast<const float*>(inline_x + a.blocks * 16 * columns) + 2 * j;
+            x_word = columns * 4;
+            x_block = 4 * x_word;
+        } else {
+            const long long x_tile = sorted.tile[m] + t0 * kPlanes / 8;
+            bx = a.x.plane + x_tile * a.blocks * 128 + lane;
+            sx = a.x.sums + x_tile * a.blocks * (kPer * 8) + 2 * j;
+            x_block = 128, x_word = 32;
+            x_step = a.blocks * 128, s_step = a.blocks * (kPer * 8);
+        }
         const int live = (n - t0) * kPlanes - g;      // of the lane's columns c * 8 + g those below
         uint4 bw[2][NT][4];
         auto fetch_x = [&](uint4 (&b)[NT][4], int kb) {
@@ -454,7 +528,11 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
                 for (int c = 0; c < NT; ++c)
                     if (c * 8 < live) {
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) b[c][w] = __ldg(bx + c * x_step + kb * 128 + w * 32);
+                        for (int w = 0; w < 4; ++w) {
+                            const uint4* from = bx + c * x_step + kb * x_block + w * x_word;
+                            if constexpr (kInline) b[c][w] = *from;
+                            else b[c][w] = __ldg(from);
+                        }
                     }
             }
         };
@@ -481,7 +559,10 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
                     for (int c = 0; c < NT; ++c)
 #pragma unroll
                         for (int q = 0; q < kPer; ++q) {
-                            const float2 v = __ldg(reinterpret_cast<const float2*>(sx + c * s_step + (kb * kPer + q) * 8));
+                            const float2* from = reinterpret_cast<const float2*>(sx + c * s_step + (kb * kPer + q) * 8);
+                            float2 v;
+                            if constexpr (kInline) v = *from;
+                            else v = __ldg(from);
                             sums[c][0][q] = v.x, sums[c][1][q] = v.y;
                         }
                 }
@@ -575,7 +656,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
         for (int i = threadIdx.x; i < out_rows * now; i += kThreads) {
             const int r = i % out_rows, token = i / out_rows;
             const int product = rows[t0 + token];
-            const float unit = __ldg(a.x.unit + a.x_share.div(product)) * (kPlanes == 2 ? 1024.0f : 1048576.0f);
+            const float unit = (kInline ? units[token] : __ldg(a.x.unit + a.x_share.div(product))) * (kPlanes == 2 ? 1024.0f : 1048576.0f);
             auto total = [&](int row) {
                 float v = 0.0f;
 #pragma unroll
@@ -666,6 +747,21 @@ int ensure_rows(MoeW4* h, int rows) {
     return MOE_OK;
 }
 
+// Lets the kernels that make operands for themselves have kInlineMax bytes.
+template <class T, int kPer> cudaError_t inline_attributes() {
+    cudaError_t e = cudaFuncSetAttribute(w4_matvec_kernel<T, 1, 1, kPer, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kInlineMax);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(w4_matvec_kernel<T, 2, 1, kPer, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kInlineMax);
+    return e;
+}
+template <int kPer> cudaError_t inline_attributes_all() {
+    cudaError_t e = inline_attributes<float, kPer>();
+    if (e == cudaSuccess) e = inline_attributes<__nv_bfloat16, kPer>();
+    if (e == cudaSuccess) e = inline_attributes<__half, kPer>();
+    return e;
+}
+
 int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, const uint8_t* zeros, MoeW4** out,
               bool on_host) {
     if (!cfg || !codes || !scales || !out) return report_error(MOE_ERR_INVALID, "moe_w4_create: null argument");
@@ -689,6 +785,8 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     int major = 0, sms = 0;
     cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, cfg->device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cfg->device);
+    if (e == cudaSuccess)
+        e = cfg->group == 128 ? inline_attributes_all<1>() : cfg->group == 64 ? inline_attributes_all<2>() : inline_attributes_all<4>();
     if (e != cudaSuccess) return launch_status(e, "moe_w4_create");
     if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_create: cannot select the device");
     if (major != 10) return report_error(MOE_ERR_UNSUPPORTED, "libmoe_b200 is built for sm_100a (B200) only");
@@ -742,14 +840,23 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     return MOE_OK;
 }
 
-template <int kPlanes, int MT, int NT>
-cudaError_t launch_product(const MoeW4* h, MatvecArgs a, int used, cudaStream_t s) {
+// Bytes of `columns` operand columns in shared memory, and whether they are
+// made there: 48 KB let two blocks stay on an SM.
+size_t inline_bytes(const MoeW4* h, int columns) {
+    return (size_t)h->blocks * (columns * 256 + kBlockK / h->cfg.group * 32);
+}
+
+template <class T, int MT, int NT, bool kInline>
+cudaError_t launch_product(const MoeW4* h, MatvecArgs a, const PlanesArgs& x, int used, int columns, bool dependent,
+                           cudaStream_t s) {
     a.groups = FastDiv((a.tiles_used + MT - 1) / MT);
     const dim3 grid((unsigned)std::min((long long)a.groups.d * used, (long long)h->sms * w4_blocks(NT))), block(w4_threads(NT));
+    const size_t smem = kInline ? inline_bytes(h, columns) : 0;
+    auto run = [&](auto kernel) { return launch(kernel, grid, block, smem, s, dependent, a, x); };
     switch (kBlockK / h->cfg.group) {
-        case 1: return launch(w4_matvec_kernel<kPlanes, MT, NT, 1>, grid, block, 0, s, true, a);
-        case 2: return launch(w4_matvec_kernel<kPlanes, MT, NT, 2>, grid, block, 0, s, true, a);
-        default: return launch(w4_matvec_kernel<kPlanes, MT, NT, 4>, grid, block, 0, s, true, a);
+        case 1: return run(w4_matvec_kernel<T, MT, NT, 1, kInline>);
+        case 2: return run(w4_matvec_kernel<T, MT, NT, 2, kInline>);
+        default: return run(w4_matvec_kernel<T, MT, NT, 4, kInline>);
     }
 }
 
@@ -757,23 +864,28 @@ template <class T>
 cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, int x_share, const int* matrix, void* y,
                     int dtype, bool dependent, cudaStream_t s) {
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
+    using Plane = std::conditional_t<kPlanes == 2, float, __half>;   // made apart, only the planes count
     const MoeW4Config& c = h->cfg;
     const int x_rows = (num_rows + x_share - 1) / x_share;
     const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1,
                        aligned16(x) && x_stride * (int64_t)sizeof(T) % 16 == 0};
-    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 1024, 0, s, dependent, p);
-    if (e != cudaSuccess) return e;
-    MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,
-                 FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
-    // Columns of a matrix's products: all rows', or twice the mean's where the rows choose their matrices.
-    const int columns = kPlanes * (matrix ? std::min(num_rows, 2 * ((num_rows + c.num_matrices - 1) / c.num_matrices)) : num_rows);
+    const MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,
+                       FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
     const int used = matrix ? std::min(num_rows, c.num_matrices) : 1;
     const long long work = (long long)a.tiles_used * used;
+    const int most = std::min(num_rows * kPlanes, 8);                // columns of a pass
+    if (num_rows <= 8 / kPlanes && inline_bytes(h, most) <= kInlineMax && work < 16ll * h->sms)
+        return work >= 3ll * h->sms || c.gated ? launch_product<T, 2, 1, true>(h, a, p, used, most, dependent, s)
+                                                : launch_product<T, 1, 1, true>(h, a, p, used, most, dependent, s);
+    cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 1024, 0, s, dependent, p);
+    if (e != cudaSuccess) return e;
+    // Columns of a matrix's products: all rows', or twice the mean's where the rows choose their matrices.
+    const int columns = kPlanes * (matrix ? std::min(num_rows, 2 * ((num_rows + c.num_matrices - 1) / c.num_matrices)) : num_rows);
     if (columns <= 8)
-        return work >= 16ll * h->sms              ? launch_product<kPlanes, 4, 1>(h, a, used, s)
-               : work >= 3ll * h->sms || c.gated ? launch_product<kPlanes, 2, 1>(h, a, used, s)
-                                                  : launch_product<kPlanes, 1, 1>(h, a, used, s);
-    return launch_product<kPlanes, 2, 2>(h, a, used, s);
+        return work >= 16ll * h->sms              ? launch_product<Plane, 4, 1, false>(h, a, p, used, 0, true, s)
+               : work >= 3ll * h->sms || c.gated ? launch_product<Plane, 2, 1, false>(h, a, p, used, 0, true, s)
+                                                  : launch_product<Plane, 1, 1, false>(h, a, p, used, 0, true, s);
+    return launch_product<Plane, 2, 2, false>(h, a, p, used, 0, true, s);
 }
 
 template <class T>
