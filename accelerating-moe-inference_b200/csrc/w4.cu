@@ -348,6 +348,7 @@ struct MatvecArgs {
     FastDiv x_share, groups;   // groups: items of a matrix
     bool gated;
     int tiles_used;         // tiles with rows of the matrix
+    int groups_part, blocks_part;   // items and blocks of 128 columns of one part; a second part's sums lie num_rows on in y
 };
 
 __device__ __forceinline__ uint4 load_stream(const uint4* p) {
@@ -363,8 +364,10 @@ __device__ __forceinline__ void store_as(void* y, long long at, float v, int dty
     else static_cast<__half*>(y)[at] = from_f32<__half>(v);
 }
 
-// y = W x.  An item is (matrix in use, MT tiles of 16 weight rows); the blocks
-// take the items in turn, a warp every kWarps-th block of 128 columns.
+// y = W x.  An item is (matrix in use, part of the columns, MT tiles of 16
+// weight rows); the thread blocks take the items in turn, a warp every
+// kWarps-th block of 128 columns.  One part is all columns; two, for results
+// that are added up anyway, even out the last turn.
 //
 // Bound by reading the weights, so a warp streams its records straight into
 // registers, four of them ahead (the first ones before the activations' kernel
@@ -403,10 +406,25 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
     uint4 code[kDepth][MT][2];
     uint32_t par[kDepth][MT][2 * kPer];
     const uint8_t* base = nullptr;     // the item's records, at the lane's place
+    // The item's matrix, tile and part of the columns: blocks [kb_first, kb_last).
+    struct Place {
+        int m, tile, part;
+    };
+    auto place_of = [&](int item) {
+        Place p;
+        p.m = a.groups.div(item);
+        const int i = item - p.m * a.groups.d;
+        p.part = i >= a.groups_part;
+        p.tile = (i - p.part * a.groups_part) * MT;
+        return p;
+    };
+    int kb_first = 0, kb_last = 0;
     auto begin = [&](int item) {
-        const int m = a.groups.div(item), tile = (item - m * a.groups.d) * MT;
-        base = a.records + ((long long)sorted.matrix[m] * (a.tiles / 4) + tile / 4) * a.blocks * (4 * kRecord) +
-               (tile % 4) * kRecord + warp * (4 * kRecord);
+        const Place p = place_of(item);
+        kb_first = p.part * a.blocks_part + warp;
+        kb_last = min(a.blocks, (p.part + 1) * a.blocks_part);
+        base = a.records + ((long long)sorted.matrix[p.m] * (a.tiles / 4) + p.tile / 4) * a.blocks * (4 * kRecord) +
+               (p.tile % 4) * kRecord + kb_first * (4 * kRecord);
     };
     // Records of the warp's d-th block of columns from `at` on; the ring's place d.
     const uint32_t code_at = lane * 16, par_at = 1024 + g * (8 * kPer);
@@ -432,7 +450,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
 #pragma unroll
         for (int d = 0; d < kDepth; ++d)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) fetch(base + d * kStep, d, t, warp + d * kWarps < a.blocks);
+            for (int t = 0; t < MT; ++t) fetch(base + d * kStep, d, t, kb_first + d * kWarps < kb_last);
     };
     int item = blockIdx.x, t0 = 0;
     if (item < items) {
@@ -495,7 +513,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
     };
 
     while (item < items) {
-        const int m = a.groups.div(item), tile = (item - m * a.groups.d) * MT;
+        const auto [m, tile, part_of] = place_of(item);
         const short* rows = sorted.rows + sorted.first[m];
         const int n = sorted.first[m + 1] - sorted.first[m];
         // The lane's part of B, and the sums of the columns whose products it
@@ -523,7 +541,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
         const int live = (n - t0) * kPlanes - g;      // of the lane's columns c * 8 + g those below
         uint4 bw[2][NT][4];
         auto fetch_x = [&](uint4 (&b)[NT][4], int kb) {
-            if (kb < a.blocks) {
+            if (kb < kb_last) {
 #pragma unroll
                 for (int c = 0; c < NT; ++c)
                     if (c * 8 < live) {
@@ -536,8 +554,8 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
                     }
             }
         };
-        fetch_x(bw[0], warp);
-        fetch_x(bw[1], warp + kWarps);
+        fetch_x(bw[0], kb_first);
+        fetch_x(bw[1], kb_first + kWarps);
 
         float y[MT][NT][kV];
 #pragma unroll
@@ -547,12 +565,12 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
 #pragma unroll
                 for (int i = 0; i < kV; ++i) y[t][c][i] = 0.0f;
 
-        for (int kb0 = warp; kb0 < a.blocks; kb0 += kUnroll * kWarps) {
+        for (int kb0 = kb_first; kb0 < kb_last; kb0 += kUnroll * kWarps) {
 #pragma unroll
             for (int d = 0; d < kUnroll; ++d) {
                 const int kb = kb0 + d * kWarps, slot = d % kDepth;
-                if (kb >= a.blocks) break;
-                const bool more = kb + kDepth * kWarps < a.blocks;
+                if (kb >= kb_last) break;
+                const bool more = kb + kDepth * kWarps < kb_last;
                 float sums[NT][2][kPer];
                 if constexpr (kPlanes == 1) {
 #pragma unroll
@@ -674,22 +692,27 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(NT)) w4_matvec_kerne
                 v = total(r);
                 out = tile * 16 + r;
             }
-            if (out < a.outputs) store_as(a.y, (long long)product * a.outputs + out, v, a.dtype);
+            if (out < a.outputs) store_as(a.y, ((long long)part_of * a.num_rows + product) * a.outputs + out, v, a.dtype);
         }
         item = next;
         t0 = next_t0;
     }
 }
 
-// y[t] = sum over s of w[t][s] * part[t * k + s], s ascending.
-template <class T> __global__ void __launch_bounds__(256) experts_sum_kernel(const float* part, const int* idx, const float* w, T* y, int k, int d, int E) {
+// y[t] = sum over s of w[t][s] * part[t * k + s], s ascending; with `second`
+// not 0 a product's second part lies that many values on.
+template <class T>
+__global__ void __launch_bounds__(256) experts_sum_kernel(const float* part, const int* idx, const float* w, T* y, int k, int d,
+                                                         int E, long long second) {
     const int n = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
     wait_predecessor_grid();
     if (n >= d) return;
     float v = 0.0f;
     for (int s = 0; s < k; ++s) {
         const int e = idx[t * k + s];
-        if (e >= 0 && e < E) v = fmaf(w[t * k + s], part[((long long)t * k + s) * d + n], v);
+        if (e < 0 || e >= E) continue;
+        const float* p = part + ((long long)t * k + s) * d + n;
+        v = fmaf(w[t * k + s], second ? p[0] + p[second] : p[0], v);
     }
     y[(long long)t * d + n] = from_f32<T>(v);
 }
@@ -704,7 +727,8 @@ struct MoeW4 {
     int outputs = 0, tiles = 0, blocks = 0, sms = 0;
     uint8_t* records = nullptr;
     Planes x{};               // the activations' operand, of work_rows rows
-    float* result = nullptr;  // fp32 results of the experts: [work_rows][outputs]
+    float* result = nullptr;  // fp32 results of the experts, result_size values
+    size_t result_size = 0;
     int work_rows = 0;
     size_t bytes = 0, work_bytes = 0;
 };
@@ -715,9 +739,7 @@ void free_work(MoeW4* h) {
     cudaFree(h->x.plane);
     cudaFree(h->x.sums);
     cudaFree(h->x.unit);
-    cudaFree(h->result);
     h->x = Planes{};
-    h->result = nullptr;
     h->bytes -= h->work_bytes;
     h->work_bytes = 0;
     h->work_rows = 0;
@@ -731,17 +753,15 @@ int ensure_rows(MoeW4* h, int rows) {
     const size_t tiles = (size_t)(2 * rows + 7) / 8 + std::min(rows, h->cfg.num_matrices) + 1;
     const size_t plane = tiles * h->blocks * 2048, unit = rows * sizeof(float);
     const size_t sums = tiles * h->blocks * (kBlockK / h->cfg.group) * 8 * sizeof(float);
-    const size_t result = (size_t)rows * h->outputs * sizeof(float);
     cudaError_t e = cudaMalloc(&h->x.plane, plane);
     if (e == cudaSuccess) e = cudaMalloc(&h->x.sums, sums);
     if (e == cudaSuccess) e = cudaMalloc(&h->x.unit, unit);
-    if (e == cudaSuccess) e = cudaMalloc(&h->result, result);
     if (e != cudaSuccess) {
         cudaGetLastError();
         free_work(h);
         return report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed");
     }
-    h->work_bytes = plane + sums + unit + result;
+    h->work_bytes = plane + sums + unit;
     h->bytes += h->work_bytes;
     h->work_rows = rows;
     return MOE_OK;
@@ -760,6 +780,23 @@ template <int kPer> cudaError_t inline_attributes_all() {
     if (e == cudaSuccess) e = inline_attributes<__nv_bfloat16, kPer>();
     if (e == cudaSuccess) e = inline_attributes<__half, kPer>();
     return e;
+}
+
+// Room for the experts' fp32 results of `rows` products, `parts` times.
+int ensure_result(MoeW4* h, int rows, int parts) {
+    const size_t n = (size_t)rows * h->outputs * parts;
+    if (n <= h->result_size) return MOE_OK;
+    cudaFree(h->result);   // waits for what still uses it
+    h->bytes -= h->result_size * sizeof(float);
+    h->result = nullptr;
+    h->result_size = 0;
+    if (cudaMalloc(&h->result, n * sizeof(float)) != cudaSuccess) {
+        cudaGetLastError();
+        return report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed");
+    }
+    h->result_size = n;
+    h->bytes += n * sizeof(float);
+    return MOE_OK;
 }
 
 int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, const uint8_t* zeros, MoeW4** out,
@@ -848,9 +885,17 @@ size_t inline_bytes(const MoeW4* h, int columns) {
 
 template <class T, int MT, int NT, bool kInline>
 cudaError_t launch_product(const MoeW4* h, MatvecArgs a, const PlanesArgs& x, int used, int columns, bool dependent,
-                           cudaStream_t s) {
-    a.groups = FastDiv((a.tiles_used + MT - 1) / MT);
-    const dim3 grid((unsigned)std::min((long long)a.groups.d * used, (long long)h->sms * w4_blocks(NT))), block(w4_threads(NT));
+                           int* parts_out, cudaStream_t s) {
+    a.groups_part = (a.tiles_used + MT - 1) / MT;
+    // Two parts where they leave the blocks' last turn fuller by a tenth.
+    const long long slots = (long long)h->sms * w4_blocks(NT), items = (long long)a.groups_part * used;
+    auto filled = [&](long long n) { return (double)n / (double)((n + slots - 1) / slots * slots); };
+    constexpr int kWarps = w4_threads(NT) / 32;
+    const int parts = parts_out && a.blocks >= 4 * kWarps && filled(2 * items) > filled(items) + 0.1 ? 2 : 1;
+    if (parts_out) *parts_out = parts;
+    a.blocks_part = (a.blocks + parts * kWarps - 1) / (parts * kWarps) * kWarps;
+    a.groups = FastDiv(parts * a.groups_part);
+    const dim3 grid((unsigned)std::min(items * parts, slots)), block(w4_threads(NT));
     const size_t smem = kInline ? inline_bytes(h, columns) : 0;
     auto run = [&](auto kernel) { return launch(kernel, grid, block, smem, s, dependent, a, x); };
     switch (kBlockK / h->cfg.group) {
@@ -862,7 +907,7 @@ cudaError_t launch_product(const MoeW4* h, MatvecArgs a, const PlanesArgs& x, in
 
 template <class T>
 cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, int x_share, const int* matrix, void* y,
-                    int dtype, bool dependent, cudaStream_t s) {
+                    int dtype, bool dependent, int* parts, cudaStream_t s) {
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     using Plane = std::conditional_t<kPlanes == 2, float, __half>;   // made apart, only the planes count
     const MoeW4Config& c = h->cfg;
@@ -870,34 +915,36 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1,
                        aligned16(x) && x_stride * (int64_t)sizeof(T) % 16 == 0};
     const MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,
-                       FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1)};
+                       FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1), 0, 0};
     const int used = matrix ? std::min(num_rows, c.num_matrices) : 1;
     const long long work = (long long)a.tiles_used * used;
     const int most = std::min(num_rows * kPlanes, 8);                // columns of a pass
     if (num_rows <= 8 / kPlanes && inline_bytes(h, most) <= kInlineMax && work < 16ll * h->sms)
-        return work >= 3ll * h->sms || c.gated ? launch_product<T, 2, 1, true>(h, a, p, used, most, dependent, s)
-                                                : launch_product<T, 1, 1, true>(h, a, p, used, most, dependent, s);
+        return work >= 3ll * h->sms || c.gated ? launch_product<T, 2, 1, true>(h, a, p, used, most, dependent, parts, s)
+                                                : launch_product<T, 1, 1, true>(h, a, p, used, most, dependent, parts, s);
     cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 1024, 0, s, dependent, p);
     if (e != cudaSuccess) return e;
     // Columns of a matrix's products: all rows', or twice the mean's where the rows choose their matrices.
     const int columns = kPlanes * (matrix ? std::min(num_rows, 2 * ((num_rows + c.num_matrices - 1) / c.num_matrices)) : num_rows);
     if (columns <= 8)
-        return work >= 16ll * h->sms              ? launch_product<Plane, 4, 1, false>(h, a, p, used, 0, true, s)
-               : work >= 3ll * h->sms || c.gated ? launch_product<Plane, 2, 1, false>(h, a, p, used, 0, true, s)
-                                                  : launch_product<Plane, 1, 1, false>(h, a, p, used, 0, true, s);
-    return launch_product<Plane, 2, 2, false>(h, a, p, used, 0, true, s);
+        return work >= 16ll * h->sms              ? launch_product<Plane, 4, 1, false>(h, a, p, used, 0, true, parts, s)
+               : work >= 3ll * h->sms || c.gated ? launch_product<Plane, 2, 1, false>(h, a, p, used, 0, true, parts, s)
+                                                  : launch_product<Plane, 1, 1, false>(h, a, p, used, 0, true, parts, s);
+    return launch_product<Plane, 2, 2, false>(h, a, p, used, 0, true, parts, s);
 }
 
 template <class T>
 cudaError_t experts_typed(MoeW4* gu, MoeW4* dn, const void* x, int tokens, int k, const int* idx, const float* w, void* y,
                           cudaStream_t s) {
+    int parts = 1;
     cudaError_t e = product(gu, static_cast<const T*>(x), tokens * k, gu->cfg.cols, k, idx, gu->result, MOE_DTYPE_F32,
-                            false, s);
+                            false, nullptr, s);
     if (e == cudaSuccess)
-        e = product(dn, gu->result, tokens * k, dn->cfg.cols, 1, idx, dn->result, MOE_DTYPE_F32, true, s);
+        e = product(dn, gu->result, tokens * k, dn->cfg.cols, 1, idx, dn->result, MOE_DTYPE_F32, true, &parts, s);
     if (e != cudaSuccess) return e;
     return launch(experts_sum_kernel<T>, dim3((dn->outputs + 255) / 256, tokens), 256, 0, s, true, dn->result, idx, w,
-                  static_cast<T*>(y), k, dn->outputs, dn->cfg.num_matrices);
+                  static_cast<T*>(y), k, dn->outputs, dn->cfg.num_matrices,
+                  parts == 2 ? (long long)tokens * k * dn->outputs : 0ll);
 }
 
 }  // namespace
@@ -929,6 +976,7 @@ void moe_w4_destroy(MoeW4* h) {
     if (!h) return;
     OnDevice on(h->cfg.device);
     cudaFree(h->records);
+    cudaFree(h->result);
     free_work(h);
     delete h;
 }
@@ -953,11 +1001,11 @@ int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_row
         if (rc != MOE_OK) return rc;
         cudaError_t e;
         if (dtype == MOE_DTYPE_F32)
-            e = product(h, static_cast<const float*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, s);
+            e = product(h, static_cast<const float*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, nullptr, s);
         else if (dtype == MOE_DTYPE_BF16)
-            e = product(h, static_cast<const __nv_bfloat16*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, s);
+            e = product(h, static_cast<const __nv_bfloat16*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, nullptr, s);
         else
-            e = product(h, static_cast<const __half*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, s);
+            e = product(h, static_cast<const __half*>(x), num_rows, x_row_stride, x_share, matrix, y, dtype, false, nullptr, s);
         return launch_status(e, "moe_w4_matvec_device");
     });
 }
@@ -983,6 +1031,8 @@ int moe_w4_experts_device(MoeW4* gu, MoeW4* dn, const void* x, int32_t dtype, in
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_experts_device: cannot select the device");
         int rc = ensure_rows(gu, T * top_k);
         if (rc == MOE_OK) rc = ensure_rows(dn, T * top_k);
+        if (rc == MOE_OK) rc = ensure_result(gu, T * top_k, 1);
+        if (rc == MOE_OK) rc = ensure_result(dn, T * top_k, 2);
         if (rc != MOE_OK) return rc;
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         cudaError_t e = dtype == MOE_DTYPE_F32    ? experts_typed<float>(gu, dn, x, T, top_k, idx, weights, y, s)

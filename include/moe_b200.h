@@ -653,7 +653,7 @@ size_t moe_w4_device_bytes(const MoeW4* h);
 
 /* y[i] = matrix[i] * x[i / x_share], i < num_rows (0..512): x
  * [ceil(num_rows / x_share)][cols] with a row stride in elements, y
- * [num_rows][outputs] contiguous, both of `dtype`.  matrix [num_rows] (device,
+ * [num_rows][outputs] contiguous, both of `dtype`, not overlapping.  matrix [num_rows] (device,
  * may be null: matrix 0): the matrix of each product; a row whose entry is
  * outside [0, num_matrices) gets zeros.  Sums are in fp32; x enters the
  * products as float16 scaled by a power of two per row: 16-bit types exactly
