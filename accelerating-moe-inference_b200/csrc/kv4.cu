@@ -285,11 +285,11 @@ __device__ __forceinline__ uint32_t quantise8(float2 (&x)[4], __half2& param) {
     if (nans) s = z = __ushort_as_half(0x7fff);
     param = __halves2half2(s, z);
     const float sf = __half2float(s), zf = __half2float(z);
-    // The quotient by the reciprocal, off by less than 1e-5; where that could
+    // The quotient by the approximate reciprocal (1 unit in the last place), off by less than 1e-5; where that could
     // change its rounding the division is done.  Adding 1.5 2^23 rounds to the
     // nearest integer, ties to even, and leaves it in the sum's low bits.
     constexpr float kRound = 12582912.0f;
-    const float inv = sf > 0.0f ? __frcp_rn(sf) : 0.0f;
+    const float inv = sf > 0.0f ? rcp_approx(sf) : 0.0f;
     const float2 down = make_float2(-zf, -zf), by = make_float2(inv, inv), round = make_float2(kRound, kRound),
                  back = make_float2(-kRound, -kRound);
     uint32_t word = 0;
@@ -362,25 +362,36 @@ template <class T, int D, bool kVec> __global__ void __launch_bounds__(D, 1024 /
         const int n = (int)(at >> 4), page = a.page.div(n);
         return a.cache + (((long long)page * a.H + head) * a.page.d + n - page * a.page.d) * kGran;
     };
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    // Token i + 8 h's pieces at `gran`, whose offsets from token i's are constants where t is i + 8 h.
+    auto put = [&](int h, uint8_t* k_at, uint8_t* v_at, uint8_t* param_at, bool store) {
         const int token = token0 + i + 8 * h;
-        const bool store = slot[h] >= 0 && slot[h] < slots;
-        const int t = whole ? i + 8 * h : (int)(slot[h] & 15);
-        uint8_t* gran = !whole && store ? granule(slot[h]) : stage;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
             __half2 param;
             const uint32_t word = quantise8(x[h][kv], param);
             if (store) {
-                *reinterpret_cast<uint32_t*>(gran + (kv == 0 ? kv4_k_word<D>(t, m) : kv4_v_word<D>(t, m))) = word;
-                if ((m & 7) == 0) *reinterpret_cast<__half2*>(gran + 16 * D + (kv * 16 + t) * G * 4 + g * 4) = param;
+                *reinterpret_cast<uint32_t*>(kv == 0 ? k_at : v_at) = word;
+                if ((m & 7) == 0) *reinterpret_cast<__half2*>(param_at + kv * 64 * G) = param;
             }
             if (a.out[kv] && token < a.N) {
                 const float v[8] = {x[h][kv][0].x, x[h][kv][0].y, x[h][kv][1].x, x[h][kv][1].y,
                                     x[h][kv][2].x, x[h][kv][2].y, x[h][kv][3].x, x[h][kv][3].y};
                 store8(static_cast<T*>(a.out[kv]) + ((long long)token * a.H + head) * D + m * 8, v);
             }
+        }
+    };
+    if (whole) {
+        uint8_t *k_at = stage + kv4_k_word<D>(i, m), *v_at = stage + kv4_v_word<D>(i, m),
+                *param_at = stage + 16 * D + i * G * 4 + g * 4;
+        put(0, k_at, v_at, param_at, true);
+        put(1, k_at + 4 * D, v_at + (G == 2 ? 512 : 8), param_at + 32 * G, true);   // token i + 8
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool store = slot[h] >= 0 && slot[h] < slots;
+            const int t = (int)(slot[h] & 15);
+            uint8_t* gran = store ? granule(slot[h]) : stage;
+            put(h, gran + kv4_k_word<D>(t, m), gran + kv4_v_word<D>(t, m), gran + 16 * D + t * G * 4 + g * 4, store);
         }
     }
     if (whole) {
