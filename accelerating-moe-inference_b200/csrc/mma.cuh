@@ -1,5 +1,5 @@
 // Warp-level pieces of the 4-bit operators: m16n8k16 products with fp32
-// accumulation and 16-byte asynchronous copies into shared memory.
+// accumulation, a transposition between lanes, approximate functions.
 //
 // Fragments of mma.m16n8k16 (lane = 4 g + j): A holds rows g, g + 8 and, per
 // register, the column pairs 2 j, 2 j + 1 (a0 row g, a1 row g + 8) and 2 j + 8,
@@ -32,23 +32,6 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// 16 bytes from global to shared memory, past L1; both addresses 16-byte aligned.
-__device__ __forceinline__ void copy16_async(uint32_t smem, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending> __device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
 // An 8x8 matrix of 16-bit elements, lane 4 g + j holding row g, columns 2 j
 // and 2 j + 1, transposed.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -57,6 +40,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return t;
 }
 
+// 1 / x within one unit in the last place, 2^x within two; subnormals as zero.
 __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
