@@ -803,7 +803,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             const unsigned have = valid >> (2 * stage) & 3;
             if (have) {
                 if (__any_sync(0xffffffffu, !mbar_wait(full + stage, phases >> stage & 1, nullptr, 0))) {
+                    // No more copies; this one gets its time once more, so that
+                    // it does not land in memory that is another block's.
                     dead = true;
+                    mbar_wait(full + stage, phases >> stage & 1, nullptr, 0);
+                    __syncwarp();
                     if (lane == 0) *a.error = kDevErrTimeoutProducer;
                 }
                 phases ^= 1u << stage;

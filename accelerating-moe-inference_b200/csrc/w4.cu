@@ -16,7 +16,9 @@ namespace {
 constexpr int kMaxRows = 512;        // products of one call
 constexpr int kBlockK = 128;         // columns of a record
 constexpr int kMaxMatrices = 256;
-constexpr int kInlineMax = 49152;    // bytes of operands that a block makes for itself
+// What a thread block makes operands of for itself: columns of x's rows times
+// blocks of 128 inputs, and bytes (two thread blocks stay on an SM).
+constexpr int kInlineBlocks = 64, kInlineMax = 49152;
 // Threads of a block and blocks of an SM, by tiles of rows and columns: what
 // the registers allow.
 __host__ __device__ constexpr int w4_threads(int NT) { return NT == 1 ? 256 : 128; }
@@ -885,8 +887,7 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     return MOE_OK;
 }
 
-// Bytes of `columns` operand columns in shared memory, and whether they are
-// made there: 48 KB let two blocks stay on an SM.
+// Bytes of `columns` operand columns in shared memory.
 size_t inline_bytes(const MoeW4* h, int columns) {
     return (size_t)h->blocks * (columns * 256 + kBlockK / h->cfg.group * 32);
 }
@@ -926,8 +927,13 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
                        FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1), 0, 0};
     const int used = matrix ? std::min(num_rows, c.num_matrices) : 1;
     const long long work = (long long)a.tiles_used * used;
+    // Two tiles of rows a block from 3 of them an SM on (one row bf16, on the GPU: 32000 x 2048 14.4 us
+    // against 16.4 with one; 4096 x 8192, 1.7 an SM, 11.2 against 10.3), four from 48 on (experts with 97 an SM
+    // 136 us against 140 with two; one row of 65536 x 4096, 28 an SM, 35.8 against 34.6).  Operands are made in every block up to kInlineBlocks (one row bf16
+    // 2048 x 2048 6.2 us against 8.2 with a kernel of their own; four rows of 4096 x 4096 12.3 against 8.3).
     const int most = std::min(num_rows * kPlanes, 8);                // columns of a pass
-    if (num_rows <= 8 / kPlanes && inline_bytes(h, most) <= kInlineMax && work < 16ll * h->sms)
+    if (num_rows <= 8 / kPlanes && x_rows * kPlanes * h->blocks <= kInlineBlocks && inline_bytes(h, most) <= kInlineMax &&
+        work < 48ll * h->sms)
         return work >= 3ll * h->sms || c.gated ? launch_product<T, 2, 1, true>(h, a, p, used, most, dependent, parts, s)
                                                 : launch_product<T, 1, 1, true>(h, a, p, used, most, dependent, parts, s);
     cudaError_t e = launch(w4_planes_kernel<T, kPlanes>, x_rows, 1024, 0, s, dependent, p);
@@ -935,7 +941,7 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     // Columns of a matrix's products: all rows', or twice the mean's where the rows choose their matrices.
     const int columns = kPlanes * (matrix ? std::min(num_rows, 2 * ((num_rows + c.num_matrices - 1) / c.num_matrices)) : num_rows);
     if (columns <= 8)
-        return work >= 16ll * h->sms              ? launch_product<Plane, 4, 1, false>(h, a, p, used, 0, true, parts, s)
+        return work >= 48ll * h->sms              ? launch_product<Plane, 4, 1, false>(h, a, p, used, 0, true, parts, s)
                : work >= 3ll * h->sms || c.gated ? launch_product<Plane, 2, 1, false>(h, a, p, used, 0, true, parts, s)
                                                   : launch_product<Plane, 1, 1, false>(h, a, p, used, 0, true, parts, s);
     // Two column tiles: one tile of rows leaves registers for a third more warps

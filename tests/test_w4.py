@@ -208,6 +208,34 @@ def test_experts(T, k, E, d, ff, group, dt):
 
 
 @pytest.mark.gpu
+@DTYPES
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K", [3968, 4096, 8064, 8192, 8320])
+@pytest.mark.parametrize("rows,share", [(1, 1), (2, 2), (4, 4), (8, 8), (2, 1)])
+def test_matvec_at_the_inline_limits(rows, share, K, group, dt):
+    """Sizes on both sides of where a product makes its operands itself: one
+    row of x that several products share, by one matrix and by several."""
+    import torch
+    pkg = load_pkg()
+    N, E = 48, 3
+    w = weights(K + group, E, N, K, group, True)
+    x = on_gpu(np.random.default_rng(K).standard_normal((-(-rows // share), K)), dt)
+    d, xd = dense(*w, group), x.double().cpu().numpy()
+    with pkg.W4Matrix(*w, group=group) as m:
+        for pick in (None, np.zeros(rows, np.int32), (np.arange(rows) % E).astype(np.int32)):
+            t = None if pick is None else torch.from_numpy(pick).cuda()
+            y = torch.full((rows, N), float("nan"), dtype=x.dtype, device="cuda")
+            m.matvec(x.data_ptr(), y.data_ptr(), rows, dt, stream(),
+                     matrix_ptr=0 if t is None else t.data_ptr(), x_share=share)
+            got = y.double().cpu().numpy()
+            for i in range(rows):
+                e = 0 if pick is None else pick[i]
+                xi = xd[i // share][None]
+                want = xi @ d[e].T
+                assert (np.abs(got[i] - want[0]) <= product_bound(d[e], xi, dt, want)[0]).all(), i
+
+
+@pytest.mark.gpu
 def test_wide_range_and_non_finite_activations():
     """fp32 activations over the whole exponent range enter exactly; an
     infinity or a NaN stays in its own row."""
