@@ -149,14 +149,21 @@ template <int kThreads, int kPlanes> __device__ void sort_products(Sorted& s, co
         const int e = __ldg(matrix + i);
         s.of[i] = (short)(e >= 0 && e < E ? e : -1);
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kThreads) {
-        int c = 0;
-        for (int i = 0; i < n; ++i) c += s.of[i] == e;
-        s.count[e] = (short)c;
-    }
+    for (int e = threadIdx.x; e < E; e += kThreads) s.count[e] = 0;
     __syncthreads();
     if (threadIdx.x < 32) {
+        // Each product's place among its matrix's, 32 products at a time.
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int i = i0 + threadIdx.x, e = i < n ? s.of[i] : -1;
+            const unsigned same = __match_any_sync(0xffffffffu, e);
+            const int rank = __popc(same & ((1u << threadIdx.x) - 1)), before = e >= 0 ? s.count[e] : 0;
+            __syncwarp();
+            if (e >= 0) {
+                s.column[i] = (short)(before + rank);
+                if (rank == 0) s.count[e] = (short)(before + __popc(same));
+            }
+            __syncwarp();
+        }
         int used = 0, at = 0, tiles = 0;
         for (int e0 = 0; e0 < E; e0 += 32) {
             const int e = e0 + threadIdx.x, c = e < E ? s.count[e] : 0;
@@ -190,8 +197,7 @@ template <int kThreads, int kPlanes> __device__ void sort_products(Sorted& s, co
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const int e = s.of[i];
         if (e < 0) continue;
-        int rank = 0;
-        for (int k = 0; k < i; ++k) rank += s.of[k] == e;
+        const int rank = s.column[i];
         s.rows[s.count[e] + rank] = (short)i;
         s.column[i] = (short)(s.tile[s.place[e]] * 8 + rank * kPlanes);
     }
