@@ -1261,6 +1261,8 @@ int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new
             return report_error(MOE_ERR_INVALID, "moe_kv4_plan_device: null pointer argument");
         if (ring_state_out == ring_state)
             return report_error(MOE_ERR_INVALID, "moe_kv4_plan_device: ring_state_out must not be ring_state");
+        if (kv_len == cached_len || kv_len == new_len)
+            return report_error(MOE_ERR_INVALID, "moe_kv4_plan_device: kv_len must not be cached_len or new_len");
         OnDevice on(c.device);
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_plan_device: cannot select the device");
         PlanArgs a{cached_len, new_len, R, c.table_width, c.block_tokens, c.num_blocks, tokens_cap, free_ring,

@@ -574,7 +574,7 @@ size_t moe_kv4_device_bytes(const MoeKv4* h);
  *                    the table holds a page outside the pool
  *   ring_state_out [2]  the state after the step (not ring_state itself)
  * Inputs are not changed other than table and ring as stated, so a step may
- * be planned again.  A ring_state outside 0 <= head < num_blocks,
+ * be planned again.  No output may overlap an input.  A ring_state outside 0 <= head < num_blocks,
  * 0 <= count <= num_blocks counts as an empty ring at 0. */
 int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new_len,
                         int32_t num_requests, int32_t* free_ring, const int32_t* ring_state,

@@ -578,6 +578,8 @@ def test_calls_refuse():
             p, p, R, p, p, tab, p, p, p, p, cap, out)
         assert bad(plan, R=0) == bad(plan, R=3) == bad(plan, cap=-1) == -1
         assert bad(plan, out=p) == bad(plan, tab=0) == -1
+        with pytest.raises(pkg.MoeError, match="kv_len"):
+            kv.plan(p, p + 64, 1, p, p, p, p, p, p, p, 1, p + 64)
         app = lambda c=p, k=p, dt=0, n=1, slot=p, out=0: kv.append(  # noqa: E731
             c, k, p, dt, n, slot, k_out_ptr=out)
         for kw in (dict(c=0), dict(c=p + 8), dict(k=0), dict(k=p + 2), dict(dt=3), dict(n=-1),
