@@ -430,6 +430,7 @@ constexpr int kAttendStages = 3;      // granule pairs in flight per warp
 constexpr int kAttendCtasPerSm = 3;
 constexpr int kAttendItemCost = 24;   // what an item costs beside its granules, in granules (measured: 25)
 constexpr int kAttendMinUnits = 12;   // a block's least share: half a pair of granules a warp more is not worth a join
+constexpr int kAttendTop = 14;        // log2 of the largest p s that a row's reference point lets stand
 constexpr int kAttendWhole = 8;       // items of up to so many granules are not cut: joining costs more
 
 // What one request asks for: its queries [q0, q0 + nq), cut length, the
@@ -780,11 +781,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
         }
 
         // Transposed outputs: lane's rows, dims 64 q + 8 g + 2 i (c0, c1) and + 1 (c2, c3).
-        float o[NT][G][4][4], m[kR], l[kR], w0[kR][G], limit[kR], room[kR], off[kR];
+        float o[NT][G][4][4], m[kR], l[kR], w0[kR][G], off[kR];
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
-            m[i] = limit[i] = -INFINITY;
-            room[i] = 2.0f / rowf[i];
+            m[i] = -INFINITY;
             l[i] = off[i] = 0.0f;
 #pragma unroll
             for (int q = 0; q < G; ++q) w0[i][q] = 0.0f;
@@ -873,6 +873,18 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                             x[i][2 * k + h] = s;
                         }
                     }
+                // Value params of the lane's tokens 16 (c / 2) + 8 (c % 2) + g.
+                uint32_t vp[4][G];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint8_t* at = st0 + (c >> 1) * kGran + 16 * D + 64 * G + (g + 8 * (c & 1)) * G * 4;
+                    if constexpr (G == 2) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(at);
+                        vp[c][0] = v.x, vp[c][1] = v.y;
+                    } else {
+                        vp[c][0] = *reinterpret_cast<const uint32_t*>(at);
+                    }
+                }
                 const int t0 = gi << 4;
                 const bool edge = have != 3 || t0 + 31 > sg.pos_lo || (a.window > 0 && t0 <= sg.pos_hi - a.window);
                 unsigned hide = 0;
@@ -889,23 +901,46 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                         }
                 }
                 // Scores are in units of 1 / rowf, rowf > 0.  The reference point m of
-                // a row's exponentials moves only when a score lies more than 2
-                // (as a power of two) above it: p stays below 4, and with a
-                // scale of at most 8736 p s stays a float16.
+                // a row's exponentials follows score + e, 2^e the power of two at
+                // or below the value's scale, so that the second product's operands
+                // p s, not p alone, fill float16's range: m moves only when one may
+                // lie above 2^14, and then so that the largest is s times a power of
+                // two, 2^12 to 2^13: it alone is rounded by next to nothing.
+                // Below 2^-14, about 2^-26 of the largest, they lose digits.
+                // Scales below 2^-14 count as 2^-15 (p stays below 2^30), a NaN or
+                // an infinity too.  Each lane asks by its own tokens' largest e.
+                __half2 big = __habs2(*reinterpret_cast<const __half2*>(&vp[0][0]));
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int q = 0; q < G; ++q) big = __hmax2(big, __habs2(*reinterpret_cast<const __half2*>(&vp[c][q])));
+                const float lift = (float)((int)(*reinterpret_cast<const uint32_t*>(&big) >> 10 & 31) - (15 + kAttendTop));
                 bool above = false;
 #pragma unroll
                 for (int i = 0; i < kR; ++i)
-                    above |= fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])) > limit[i];
+                    above |= fmaf(fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])), rowf[i], lift) > m[i];
                 if (__any_sync(0xffffffffu, above)) {
+                    float e[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        int field = 0;
+#pragma unroll
+                        for (int q = 0; q < G; ++q) {
+                            const int f = vp[c][q] >> 10 & 31;
+                            field = max(field, f == 31 ? 0 : f);
+                        }
+                        e[c] = (float)(field - (15 + kAttendTop));
+                    }
 #pragma unroll
                     for (int i = 0; i < kR; ++i) {
-                        float top = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) top = fmaxf(top, fmaf(x[i][c], rowf[i], e[c]));
 #pragma unroll
                         for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                        const float keep = top > m[i] ? exp2_approx((m[i] - top) * rowf[i]) : 1.0f;
-                        m[i] = fmaxf(m[i], top);
-                        limit[i] = m[i] + room[i];
-                        off[i] = m[i] == -INFINITY ? 0.0f : m[i] * rowf[i];
+                        if (!(top > m[i])) continue;     // the same in the row's lanes
+                        const float to = top + 2.0f, keep = exp2_approx(m[i] - to);
+                        m[i] = off[i] = to;
                         l[i] *= keep;
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
@@ -934,17 +969,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 auto weigh = [&](auto at_edge) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t vp[G];
-                        const uint8_t* at = st0 + (c >> 1) * kGran + 16 * D + 64 * G + (g + 8 * (c & 1)) * G * 4;
-                        if constexpr (G == 2) {
-                            const uint2 v = *reinterpret_cast<const uint2*>(at);
-                            vp[0] = v.x, vp[1] = v.y;
-                        } else {
-                            vp[0] = *reinterpret_cast<const uint32_t*>(at);
-                        }
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
-                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&vp[q]));
+                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&vp[c][q]));
                             float v[kR];
 #pragma unroll
                             for (int i = 0; i < kR; ++i) {
@@ -1050,8 +1077,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             T t[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
             if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(t);
             else *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(t);
-            if (a.lse && d == 0)
-                a.lse[at] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+            if (a.lse && d == 0) {   // l may be 2^40: its power of two goes to m
+                const int e = min(max((int)(__float_as_uint(ll) >> 23) - 127, -126), 126);
+                a.lse[at] = ll == 0.0f ? -INFINITY
+                                       : ((mm + (float)e) + log2f(ll * __uint_as_float((127 - e) << 23))) * 0.6931471805599453f;
+            }
         };
         for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
             const int row = i / (D / 4), d = i % (D / 4) * 4;
