@@ -459,13 +459,16 @@ template <int kRows> __device__ __forceinline__ Request request_of(const AttendA
 // a pair of subnormals (c 2^-24, or c 2^-20 from the higher nibble of a byte):
 // exact, but the tensor core aligns a subnormal's products by its exponent
 // field, 2^3 to 2^10 above its value, and drops that much of the sum's low end
-// (measured: 5e-6 of the result's norm).  kNormal: made normal by one exact
-// multiplication by 2^14.
+// (measured: 5e-6 of the result's norm).  kNormal: made the normal number
+// (c - 8) 2^14 times that by one exact fma.  Counted from the middle the terms
+// have both signs: a sum of c alone grows to many times the result and is cut
+// down to it by the minimums' sum, and what each step of it cut off shows (64
+// requests of 100 to 8192 keys: 4e-6 of the result's norm, 1.6e-7 with c - 8).
 template <bool kNormal> __device__ __forceinline__ uint32_t codes(uint32_t word, uint32_t mask) {
     uint32_t v = word & mask;
     if constexpr (kNormal) {
-        const __half2 k = __float2half2_rn(16384.0f);
-        const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), k);
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(16384.0f),
+                                  __float2half2_rn(mask == 0x000f000fu ? -8.0f / 1024.0f : -8.0f / 64.0f));
         v = *reinterpret_cast<const uint32_t*>(&r);
     }
     return v;
@@ -552,6 +555,7 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 //   q . k = s (q . c) + m sum(q),
 // those of a value go into the probabilities before the second product,
 //   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t m_t.
+// fp32: with c - 8 in the place of c and m + 8 s in that of m.
 // fp32 queries take two float16 planes, hi and (x - hi) 2^11, as neighbouring
 // columns of the same product (22 bits); so do their probabilities.
 //
@@ -867,7 +871,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                                 const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
                                 const float (&t)[4] = acc[k][i / kE][q];
                                 const float d = kPlanes == 2 ? fmaf(t[2 * h + 1], kLo, t[2 * h]) : t[2 * h + i % kE];
-                                s = q == 0 ? p.y * qs[i][q] : fmaf(p.y, qs[i][q], s);
+                                const float zero = kNormal ? fmaf(p.x, 8.0f, p.y) : p.y;
+                                s = q == 0 ? zero * qs[i][q] : fmaf(zero, qs[i][q], s);
                                 s = fmaf(p.x, d, s);
                             }
                             x[i][2 * k + h] = s;
@@ -971,7 +976,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                     for (int c = 0; c < 4; ++c) {
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
-                            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&vp[c][q]));
+                            float2 p = __half22float2(*reinterpret_cast<const __half2*>(&vp[c][q]));
+                            if constexpr (kNormal) p.y = fmaf(p.x, 8.0f, p.y);
                             float v[kR];
 #pragma unroll
                             for (int i = 0; i < kR; ++i) {

@@ -166,3 +166,34 @@ def test_groups_of_different_size(dt):
     if dt == 2:
         small += 2.0 ** -25 * (want[..., 64:].numel() ** 0.5 / want[..., 64:].norm().item())
     assert e.item() <= small
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,nq", [(1, 1), (2, 3)])
+def test_fp32_sums_of_evenly_shared_values(H, nq, D):
+    """Short queries give thousands of keys nearly the same probability, so that
+    an fp32 result is a mean of their values, far smaller than each, and its
+    sum's roundings are most of what is left.  Terms counted from the middle of
+    the codes, p s (c - 8), have both signs: a warp's sum of 16 j of them is
+    about 12 sqrt(j) s p, and its steps' losses, 2^-24 of that each and of either
+    sign, are together 2^-24 * 12 s p L / 64 / sqrt(2); four warps, p = 1 / L:
+    0.27 * 2^-24 s.  Eight times that, and 2^-21 on each p v for the scores (below
+    2) and their exponentials."""
+    import torch
+    # So many that a block has a whole item or more: runs of 64 steps a warp.
+    b = batch(0, D, H=H * 8, Hkv=8, lens=(4096,) * 24, nqs=(nq,) * 24, bs=64)
+    k, v = keys_and_values(b)
+    refill(b, k, v)
+    b.q.mul_(0.3)
+    out, _ = b.run()
+    want, *_ = exact(b)
+    scale = []
+    for r in range(b.R):
+        x = b.v[int(b.first[r]):int(b.first[r + 1])].double().unflatten(-1, (-1, 64))
+        s = (x.amax(-1) - x.amin(-1)).square().mean((0, 1)).sqrt() / 15      # a group's rms step
+        scale.append(s.repeat_interleave(64).expand(nq, b.H, D))
+    # || (sum (p v)^2)^(1/2) || is the result's own norm, its values being independent.
+    tol = 2.0 ** -23 * torch.cat(scale).norm().item() + 2.0 ** -21 * want.norm().item()
+    err = (out.double() - want).norm().item()
+    assert err <= tol, (err / want.norm().item(), tol / want.norm().item())
