@@ -556,17 +556,23 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // those of a value go into the probabilities before the second product,
 //   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t m_t.
 // fp32: with c - 8 in the place of c and m + 8 s in that of m.
-// fp32 queries take two float16 planes, hi and (x - hi) 2^11, as neighbouring
-// columns of the same product (22 bits); so do their probabilities.
+// Two planes: fp32 queries, and any type's p s, enter as two float16 numbers, hi
+// and (x - hi) 2^11, in neighbouring columns of the same product (22 bits).
+// 16-bit types take them where up to four rows leave the columns free, which
+// halves the softmax's work too (a lane has one row instead of two: attend_long
+// 118 us with one plane, 113 with two).  With one plane p s has 11 bits, and so
+// that its rounding counts on c - 7.5 only, not on c, a product with ones gives
+// the rounded numbers' sum: sum (p s)~ c - 7.5 sum (p s)~ + sum p (m + 7.5 s)
+// (float16 results of 8 rows and 100 to 2048 keys: 1.13 times what their own
+// rounding leaves instead of 1.75, at no cost that shows).
 //
 // Bound by its instructions, about 270 a granule of 2304 bytes at two a cycle.
 // 8 requests of 16 k to 131 k tokens, 32 query and 8 key/value heads of 128,
 // f16: 112 to 122 us, 509 MB at 4.2 to 4.5 TB/s (the copies alone: 85 us); 64
 // requests of 100 to 8192, bf16: 47 us; one of 640, 16 heads, fp32: 12 us.
 // NT: column tiles of 8; two take 16 query rows (fp32: 8) per unpacking.
-template <class T, int D, int NT>
+template <class T, int D, int NT, int kPlanes>
 __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm : 2) attend_kernel(AttendArgs a) {
-    constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     constexpr int kRows = 8 * NT / kPlanes;    // query rows of a tile
     constexpr int kE = 2 / kPlanes;            // rows per lane and column tile
     constexpr int kR = kE * NT;                // rows per lane
@@ -575,8 +581,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     constexpr int kPitch = D + 4;              // floats per output row in shared memory
     constexpr int kThreads = kAttendWarps * 32;
     constexpr float kLo = 1.0f / 2048.0f;      // weight of the low plane
-    constexpr bool kNormal = kPlanes == 2;     // fp32 results need the whole of their sums
+    constexpr bool kNormal = sizeof(T) == 4;   // fp32 results need the whole of their sums
     constexpr float kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
+    constexpr float kCentre = kNormal ? 8.0f : kPlanes == 1 ? 7.5f : 0.0f;   // the code that values are counted from
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     constexpr int kStage = 2 * kGran;
     constexpr int kWarpFloats = kRows * kPitch + 2 * kRows;   // a warp's result
@@ -785,7 +792,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
         }
 
         // Transposed outputs: lane's rows, dims 64 q + 8 g + 2 i (c0, c1) and + 1 (c2, c3).
-        float o[NT][G][4][4], m[kR], l[kR], w0[kR][G], off[kR];
+        float o[NT][G][4][4], all[NT][G][4], m[kR], l[kR], w0[kR][G], off[kR];
 #pragma unroll
         for (int i = 0; i < kR; ++i) {
             m[i] = -INFINITY;
@@ -798,9 +805,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
             for (int q = 0; q < G; ++q)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int c = 0; c < 4; ++c) {
+                    all[n][q][c] = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) o[n][q][i][c] = 0.0f;
+                    for (int i = 0; i < 4; ++i) o[n][q][i][c] = 0.0f;
+                }
 
         for (int gi = sg.ga + 2 * warp; gi < sg.gb; gi += 2 * kAttendWarps) {
             const uint8_t* st0 = ring + stage * kStage;
@@ -950,6 +959,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
                             w0[i][q] *= keep;
+                            if constexpr (kPlanes == 1) {
+                                all[i / kE][q][i % kE] *= keep;
+                                all[i / kE][q][2 + i % kE] *= keep;
+                            }
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 float (&t)[4] = o[i / kE][q][k];
@@ -977,7 +990,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
                             float2 p = __half22float2(*reinterpret_cast<const __half2*>(&vp[c][q]));
-                            if constexpr (kNormal) p.y = fmaf(p.x, 8.0f, p.y);
+                            if constexpr (kCentre != 0.0f) p.y = fmaf(p.x, kCentre, p.y);
                             float v[kR];
 #pragma unroll
                             for (int i = 0; i < kR; ++i) {
@@ -1022,7 +1035,12 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                         vw[0][0][0] = v.x, vw[0][1][0] = v.y, vw[1][0][0] = v.z, vw[1][1][0] = v.w;
                     }
 #pragma unroll
-                    for (int q = 0; q < G; ++q)
+                    for (int q = 0; q < G; ++q) {
+                        if constexpr (kPlanes == 1) {
+                            constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(all[n][q], kOnes, pb[k][n][q][0], pb[k][n][q][1]);
+                        }
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {   // byte i: nibbles 2 i (rows g) and 2 i + 1 (rows g + 8)
                             const uint32_t sel = 0x0400 + 0x0101 * i;
@@ -1033,6 +1051,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                             for (int n = 0; n < NT; ++n) mma_f16(o[n][q][i], f, pb[k][n][q][0], pb[k][n][q][1]);
                         }
+                    }
                 }
             }
             __syncwarp();
@@ -1052,6 +1071,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 float z = w0[i][q];
 #pragma unroll
                 for (int k = 4; k < 32; k <<= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
+                if constexpr (kPlanes == 1) z = fmaf(all[i / kE][q][i % kE], -kCentre, z);
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -1162,16 +1182,23 @@ using namespace moe;
 namespace {
 
 // The warps' rings, then their results.
-template <class T, int D, int NT> constexpr int attend_smem_bytes() {
-    return kAttendWarps * (kAttendStages * 2 * kv4_granule(D) + 8 * NT / (sizeof(T) == 4 ? 2 : 1) * (D + 4 + 2) * 4);
+template <int D, int NT, int kPlanes> constexpr int attend_smem_bytes() {
+    return kAttendWarps * (kAttendStages * 2 * kv4_granule(D) + 8 * NT / kPlanes * (D + 4 + 2) * 4);
+}
+
+template <class T, int D, int NT, int kPlanes> cudaError_t attend_attribute() {
+    return cudaFuncSetAttribute(attend_kernel<T, D, NT, kPlanes>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                attend_smem_bytes<D, NT, kPlanes>());
 }
 
 template <class T, int D> cudaError_t attend_attributes_of() {
-    cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         attend_smem_bytes<T, D, 1>());
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(attend_kernel<T, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 attend_smem_bytes<T, D, 2>());
+    cudaError_t e = attend_attribute<T, D, 1, 2>();
+    if constexpr (sizeof(T) == 4) {
+        if (e == cudaSuccess) e = attend_attribute<T, D, 2, 2>();
+    } else {
+        if (e == cudaSuccess) e = attend_attribute<T, D, 1, 1>();
+        if (e == cudaSuccess) e = attend_attribute<T, D, 2, 1>();
+    }
     return e;
 }
 
@@ -1326,13 +1353,18 @@ template <class T> cudaError_t append_dim(const AppendArgs& a, int D, bool vec, 
     return D == 64 ? append_typed<T, 64>(a, vec, s) : append_typed<T, 128>(a, vec, s);
 }
 
+template <class T, int D, int NT, int kPlanes> cudaError_t attend_launch(const AttendArgs& a, int sms, cudaStream_t s) {
+    return launch(attend_kernel<T, D, NT, kPlanes>, sms * (NT == 1 ? kAttendCtasPerSm : 2), dim3(kAttendWarps * 32),
+                  attend_smem_bytes<D, NT, kPlanes>(), s, false, a);
+}
+
 template <class T, int D> cudaError_t attend_tiles(const AttendArgs& a, int sms, cudaStream_t s) {
-    const dim3 block(kAttendWarps * 32);
-    // Columns that a request's queries of one key/value head need on average.
-    const long long columns = (long long)(a.H / a.Hkv) * ((a.tokens + a.R - 1) / a.R) * (sizeof(T) == 4 ? 2 : 1);
-    return columns <= 8
-               ? launch(attend_kernel<T, D, 1>, sms * kAttendCtasPerSm, block, attend_smem_bytes<T, D, 1>(), s, false, a)
-               : launch(attend_kernel<T, D, 2>, sms * 2, block, attend_smem_bytes<T, D, 2>(), s, false, a);
+    // Rows that a request's queries of one key/value head have on average.  Up to 4 the 8 columns
+    // of a product hold two planes of each (why at attend_kernel).
+    const long long rows = (long long)(a.H / a.Hkv) * ((a.tokens + a.R - 1) / a.R);
+    if (rows <= 4) return attend_launch<T, D, 1, 2>(a, sms, s);
+    if constexpr (sizeof(T) == 4) return attend_launch<T, D, 2, 2>(a, sms, s);
+    else return rows <= 8 ? attend_launch<T, D, 1, 1>(a, sms, s) : attend_launch<T, D, 2, 1>(a, sms, s);
 }
 
 template <class T> cudaError_t attend_dim(const AttendArgs& a, int D, int sms, cudaStream_t s) {

@@ -609,10 +609,12 @@ int moe_kv4_append_device(MoeKv4* h, void* cache, const void* k, const void* v, 
  * tokens behind q_offset[num_requests] are not written.  kv_len beyond the
  * table's width is cut to it; keys on a page outside the pool are not seen.
  * Scores, softmax and sums are in fp32.  q enters its product as float16 with
- * 11 significant bits for 16-bit types and 22 for fp32; so does, for each key
- * and group of 64 dims, its probability times the value's scale, as long as it
- * is above 2^-26 of the row's largest (scales below 2^-14 count as that), below
- * that with a step of 2^-36 of the largest (fp32: 2^-47).  The kernel's waits are bounded; once one has run out (its results are
+ * 11 significant bits for 16-bit types and 22 for fp32.  For each key and group
+ * of 64 dims its probability times the value's scale enters as float16 with 22
+ * significant bits, with 11 for 16-bit types where requests have on average
+ * more than four rows (queries times num_heads / num_kv_heads) a key/value
+ * head, as long as it is above 2^-26 of the row's largest (scales below 2^-14
+ * count as that), and below that with a step of 2^-47 (2^-36) of the largest.  The kernel's waits are bounded; once one has run out (its results are
  * then undefined), every later call on the handle returns MOE_ERR_TIMEOUT. */
 int moe_kv4_attention_device(MoeKv4* h, const void* cache, const void* q, int32_t dtype,
                              int32_t tokens, int32_t num_heads, int64_t q_token_stride,

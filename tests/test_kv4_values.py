@@ -197,3 +197,26 @@ def test_fp32_sums_of_evenly_shared_values(H, nq, D):
     tol = 2.0 ** -23 * torch.cat(scale).norm().item() + 2.0 ** -21 * want.norm().item()
     err = (out.double() - want).norm().item()
     assert err <= tol, (err / want.norm().item(), tol / want.norm().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,nq", [(4, 1, 1), (2, 2, 3), (6, 1, 1), (8, 1, 1), (4, 1, 2), (16, 1, 1), (8, 2, 4)])
+@pytest.mark.parametrize("dt", [1, 2], ids=["bf16", "f16"])
+def test_16_bit_results_are_as_good_as_their_type(H, Hkv, nq, dt):
+    """A result rounded once from an exact one is off by a relative error that is
+    spread evenly, 2^-bits at most.  What the probabilities' rounding adds is
+    nothing to speak of with two float16 numbers each (up to four rows a
+    key/value head); with one, an error spread alike on each p s (c - 7.5), which
+    is the value but for the middle of its group's range: as much as a float16
+    result's own, 1.5 times that with room for the middle.  So the total stays
+    below 1.5 times the own rounding's norm, and below sqrt(1 + 1.5^2) times for
+    float16 results with one number."""
+    b = batch(dt, 128, H=H, Hkv=Hkv, lens=(2048, 700, 1500), nqs=(nq,) * 3, bs=32)
+    k, v = keys_and_values(b)
+    refill(b, k, v)
+    out, _ = b.run()
+    want, *_ = exact(b)
+    once = (want.to(b.q.dtype).double() - want).norm().item()
+    most = 1.5 if dt == 1 or H // Hkv * nq <= 4 else (1 + 1.5 ** 2) ** 0.5
+    err = (out.double() - want).norm().item()
+    assert err <= most * once, (err / once, most)
