@@ -65,6 +65,8 @@ struct PlanArgs {
 };
 
 constexpr int kPlanThreads = 1024;
+constexpr int kMaxRequests = 8192;
+constexpr size_t plan_smem_bytes(int R) { return (size_t)(2 * R + 1) * sizeof(int); }
 
 // Every block scans all requests (R <= 8192 lengths, L2-resident), so that no
 // block waits for another; the requests' rows and the tokens are then split
@@ -1252,7 +1254,7 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
             (long long)cfg->table_width * cfg->block_tokens > (1 << 30))
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: need num_blocks >= 1, table_width >= 1 and "
                                                  "table_width * block_tokens <= 2^30");
-        if (cfg->max_requests < 1 || cfg->max_requests > 8192)
+        if (cfg->max_requests < 1 || cfg->max_requests > kMaxRequests)
             return report_error(MOE_ERR_INVALID, "moe_kv4_create: max_requests must be 1..8192");
         int ndev = 0;
         if (cudaGetDeviceCount(&ndev) != cudaSuccess || cfg->device < 0 || cfg->device >= ndev)
@@ -1261,9 +1263,10 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
         int major = 0, sms = 0;
         cudaError_t e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, cfg->device);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cfg->device);
+        // The kernel's limit, not the handle's: every handle asks for the same.
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (2 * cfg->max_requests + 1) * (int)sizeof(int));
+                                     (int)plan_smem_bytes(kMaxRequests));
         if (e == cudaSuccess) e = attend_attributes(cfg->head_dim);
         if (e != cudaSuccess) return launch_status(e, "moe_kv4_create");
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_create: cannot select the device");
@@ -1331,7 +1334,7 @@ int moe_kv4_plan_device(MoeKv4* h, const int32_t* cached_len, const int32_t* new
         PlanArgs a{cached_len, new_len, R, c.table_width, c.block_tokens, c.num_blocks, tokens_cap, free_ring,
                    ring_state, block_table, kv_len, q_offset, position,
                    reinterpret_cast<long long*>(slot), ring_state_out, FastDiv(c.block_tokens)};
-        const size_t smem = (size_t)(2 * R + 1) * sizeof(int);
+        const size_t smem = plan_smem_bytes(R);
         // A thread per token, a block for every 64 requests' rows, one block per SM at most.
         const int grid = std::max(1, std::min(h->sms, std::max(tokens_cap / kPlanThreads + 1, (R + 63) / 64)));
         return launch_status(launch(plan_kernel, grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream), false, a),
