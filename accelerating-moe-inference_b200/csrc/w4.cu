@@ -4,6 +4,7 @@
 #include <cstring>
 #include <type_traits>
 #include <new>
+#include <vector>
 
 #include "dtype.cuh"
 #include "mma.cuh"
@@ -746,39 +747,49 @@ struct MoeW4 {
     float* result = nullptr;  // fp32 results of the experts, result_size values
     size_t result_size = 0;
     int work_rows = 0;
-    size_t bytes = 0, work_bytes = 0;
+    std::vector<void*> held;  // the workspaces, outgrown ones too: enqueued work and graphs name them
+    size_t bytes = 0;
 };
 
 namespace {
 
-void free_work(MoeW4* h) {
-    cudaFree(h->x.plane);
-    cudaFree(h->x.sums);
-    cudaFree(h->x.unit);
-    h->x = Planes{};
-    h->bytes -= h->work_bytes;
-    h->work_bytes = 0;
-    h->work_rows = 0;
+// A further workspace.  Nothing is freed before the handle is, and nothing
+// waited for: what is enqueued or was captured with a smaller one keeps it.
+int hold(MoeW4* h, size_t bytes, cudaStream_t s, uint8_t** out) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &capture) != cudaSuccess) cudaGetLastError();
+    else if (capture != cudaStreamCaptureStatusNone)
+        return report_error(MOE_ERR_UNSUPPORTED, "4-bit weights: this call needs more workspace than the handle has, which a "
+                                                 "stream capture does not allow; create it with a larger max_rows, or make a "
+                                                 "call of this size before the capture");
+    h->held.reserve(h->held.size() + 1);
+    void* p = nullptr;
+    const cudaError_t e = cudaMalloc(&p, bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed")
+                                              : launch_status(e, "4-bit weights: workspace allocation");
+    }
+    h->held.push_back(p);
+    h->bytes += bytes;
+    *out = static_cast<uint8_t*>(p);
+    return MOE_OK;
 }
 
-int ensure_rows(MoeW4* h, int rows) {
+// Operands for `rows` products; a handle that outgrows its own at least doubles
+// them, so that what it holds stays below twice the last.
+int ensure_rows(MoeW4* h, int rows, cudaStream_t s) {
     if (rows <= h->work_rows) return MOE_OK;
-    free_work(h);   // waits for what still uses it
+    rows = std::max(rows, std::min(2 * h->work_rows, kMaxRows));
     // Column tiles: two columns a product, one not full for each matrix in use,
     // and one that the last pass of a kernel of two column tiles may look at.
     const size_t tiles = (size_t)(2 * rows + 7) / 8 + std::min(rows, h->cfg.num_matrices) + 1;
     const size_t plane = tiles * h->blocks * 2048, unit = rows * sizeof(float);
-    const size_t sums = tiles * h->blocks * (kBlockK / h->cfg.group) * 8 * sizeof(float);
-    cudaError_t e = cudaMalloc(&h->x.plane, plane);
-    if (e == cudaSuccess) e = cudaMalloc(&h->x.sums, sums);
-    if (e == cudaSuccess) e = cudaMalloc(&h->x.unit, unit);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        free_work(h);
-        return report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed");
-    }
-    h->work_bytes = plane + sums + unit;
-    h->bytes += h->work_bytes;
+    const size_t sums = tiles * h->blocks * (kBlockK / h->cfg.group) * 8 * sizeof(float);   // a multiple of 32
+    uint8_t* at = nullptr;
+    const int rc = hold(h, plane + sums + unit, s, &at);
+    if (rc != MOE_OK) return rc;
+    h->x = Planes{reinterpret_cast<uint4*>(at), reinterpret_cast<float*>(at + plane), reinterpret_cast<float*>(at + plane + sums)};
     h->work_rows = rows;
     return MOE_OK;
 }
@@ -798,20 +809,17 @@ template <int kPer> cudaError_t inline_attributes_all() {
     return e;
 }
 
-// Room for the experts' fp32 results of `rows` products, `parts` times.
-int ensure_result(MoeW4* h, int rows, int parts) {
-    const size_t n = (size_t)rows * h->outputs * parts;
-    if (n <= h->result_size) return MOE_OK;
-    cudaFree(h->result);   // waits for what still uses it
-    h->bytes -= h->result_size * sizeof(float);
-    h->result = nullptr;
-    h->result_size = 0;
-    if (cudaMalloc(&h->result, n * sizeof(float)) != cudaSuccess) {
-        cudaGetLastError();
-        return report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed");
-    }
+// Room for the experts' fp32 results of `rows` products: two parts where the
+// product may be split (launch_product), which is the down product.
+int ensure_result(MoeW4* h, int rows, cudaStream_t s) {
+    const size_t row = (size_t)h->outputs * (h->cfg.gated ? 1 : 2);
+    if (rows * row <= h->result_size) return MOE_OK;
+    const size_t n = std::max(rows * row, std::min(2 * h->result_size, kMaxRows * row));
+    uint8_t* at = nullptr;
+    const int rc = hold(h, n * sizeof(float), s, &at);
+    if (rc != MOE_OK) return rc;
+    h->result = reinterpret_cast<float*>(at);
     h->result_size = n;
-    h->bytes += n * sizeof(float);
     return MOE_OK;
 }
 
@@ -883,7 +891,9 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     cudaFree(stage);
     int rc = e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed")
                                             : launch_status(e, "moe_w4_create");
-    if (rc == MOE_OK) rc = ensure_rows(h, cfg->max_rows);
+    if (rc == MOE_OK) rc = ensure_rows(h, cfg->max_rows, nullptr);
+    // The experts' matrices; others are not asked for results of that kind.
+    if (rc == MOE_OK && (cfg->gated || cfg->num_matrices > 1)) rc = ensure_result(h, cfg->max_rows, nullptr);
     if (rc != MOE_OK) {
         cudaGetLastError();
         moe_w4_destroy(h);
@@ -999,8 +1009,7 @@ void moe_w4_destroy(MoeW4* h) {
     if (!h) return;
     OnDevice on(h->cfg.device);
     cudaFree(h->records);
-    cudaFree(h->result);
-    free_work(h);
+    for (void* p : h->held) cudaFree(p);
     delete h;
 }
 
@@ -1020,7 +1029,7 @@ int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_row
         OnDevice on(h->cfg.device);
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_matvec_device: cannot select the device");
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const int rc = ensure_rows(h, num_rows);
+        const int rc = ensure_rows(h, num_rows, s);
         if (rc != MOE_OK) return rc;
         cudaError_t e;
         if (dtype == MOE_DTYPE_F32)
@@ -1052,12 +1061,12 @@ int moe_w4_experts_device(MoeW4* gu, MoeW4* dn, const void* x, int32_t dtype, in
             return report_error(MOE_ERR_INVALID, "moe_w4_experts_device: x and y must be aligned to their elements");
         OnDevice on(gu->cfg.device);
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_experts_device: cannot select the device");
-        int rc = ensure_rows(gu, T * top_k);
-        if (rc == MOE_OK) rc = ensure_rows(dn, T * top_k);
-        if (rc == MOE_OK) rc = ensure_result(gu, T * top_k, 1);
-        if (rc == MOE_OK) rc = ensure_result(dn, T * top_k, 2);
-        if (rc != MOE_OK) return rc;
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        int rc = ensure_rows(gu, T * top_k, s);
+        if (rc == MOE_OK) rc = ensure_rows(dn, T * top_k, s);
+        if (rc == MOE_OK) rc = ensure_result(gu, T * top_k, s);
+        if (rc == MOE_OK) rc = ensure_result(dn, T * top_k, s);
+        if (rc != MOE_OK) return rc;
         cudaError_t e = dtype == MOE_DTYPE_F32    ? experts_typed<float>(gu, dn, x, T, top_k, idx, weights, y, s)
                         : dtype == MOE_DTYPE_BF16 ? experts_typed<__nv_bfloat16>(gu, dn, x, T, top_k, idx, weights, y, s)
                                                   : experts_typed<__half>(gu, dn, x, T, top_k, idx, weights, y, s);

@@ -636,13 +636,21 @@ typedef struct MoeW4Config {
     int32_t group;         /* 32, 64 or 128 */
     int32_t gated;
     int32_t device;
-    int32_t max_rows;      /* workspace is pre-sized for this many product rows; grows on demand */
+    int32_t max_rows;      /* workspace is pre-sized for this many product rows; see below */
     int32_t reserved[5];
 } MoeW4Config;
 
 typedef struct MoeW4 MoeW4;
 
-/* One matrix of 4096 x 4096, group 128, device 0, 16 product rows. */
+/* A handle holds the weights in its own layout and a workspace: one stream at
+ * a time, replays of captured calls included.  The workspace is pre-sized for
+ * max_rows product rows (num_rows, or num_tokens * top_k), with the experts'
+ * fp32 results where the matrix is gated or num_matrices > 1.  A call that needs
+ * more allocates it; what it outgrows is freed with the handle only, so earlier
+ * captures of the handle's calls stay good.  Such a call inside a stream
+ * capture returns MOE_ERR_UNSUPPORTED and leaves the capture as it was.
+ *
+ * One matrix of 4096 x 4096, group 128, device 0, 16 product rows. */
 void moe_w4_config_init(MoeW4Config* cfg);
 /* From codes [num_matrices][rows][cols / 2] (two codes per byte, the even
  * column in the low nibble), scales [num_matrices][rows][ceil(cols / group)]
