@@ -2,8 +2,11 @@
 // quantising append, and attention over the cache.
 #include <algorithm>
 #include <cmath>
+#include <memory>
+#include <mutex>
 #include <new>
 #include <type_traits>
+#include <vector>
 
 #include "dtype.cuh"
 #include "kv4.cuh"
@@ -1219,10 +1222,53 @@ struct MoeKv4 {
     MoeKv4Config cfg;
     int sms = 0;
     float* part = nullptr;     // attention: partial rows of items that several blocks share
-    int* counter = nullptr;
+    int* counter = nullptr;    // behind them
     int* error = nullptr;      // pinned host memory: a kernel's wait ran out
     size_t bytes = 0;
 };
+
+namespace {
+
+// The handles' error words.  Pinning memory costs milliseconds, so they share
+// pages that stay the process's; a word is given back only after its device has
+// no work of the handle left.
+class ErrorWords {
+public:
+    cudaError_t take(int** out) {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (free_.empty()) {
+            constexpr int kWords = 1024;
+            free_.reserve(kWords * (pages_ + 1));    // giving one back never allocates
+            int* page = nullptr;
+            const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&page), kWords * sizeof(int),
+                                                cudaHostAllocMapped | cudaHostAllocPortable);
+            if (e != cudaSuccess) return e;
+            ++pages_;
+            for (int i = 0; i < kWords; ++i) free_.push_back(page + i);
+        }
+        *out = free_.back();
+        free_.pop_back();
+        **out = 0;
+        return cudaSuccess;
+    }
+    void give(int* word) {
+        if (!word) return;
+        std::lock_guard<std::mutex> lock(mutex_);
+        free_.push_back(word);
+    }
+
+private:
+    std::mutex mutex_;
+    std::vector<int*> free_;
+    size_t pages_ = 0;
+};
+
+ErrorWords& error_words() {
+    static ErrorWords* words = new ErrorWords;    // not destroyed: handles may be, at the process's end
+    return *words;
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -1272,26 +1318,26 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
         if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_kv4_create: cannot select the device");
         if (major != 10)
             return report_error(MOE_ERR_UNSUPPORTED, "libmoe_b200 is built for sm_100a (B200) only");
-        auto* h = new MoeKv4;
+        std::unique_ptr<MoeKv4, void (*)(MoeKv4*)> h(new MoeKv4, moe_kv4_destroy);
         h->cfg = *cfg;
         h->sms = sms;
         const size_t grid = (size_t)sms * kAttendCtasPerSm;
         const size_t part = grid * 2 * 16 * (cfg->head_dim + 2) * sizeof(float);
         const size_t counter = grid * sizeof(int);
-        e = cudaMalloc(&h->part, part);
-        if (e == cudaSuccess) e = cudaMalloc(&h->counter, counter);
-        if (e == cudaSuccess) e = cudaMemset(h->counter, 0, counter);
+        e = cudaMalloc(&h->part, part + counter);
+        if (e == cudaSuccess) {
+            h->counter = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(h->part) + part);
+            e = cudaMemset(h->counter, 0, counter);
+        }
         if (e == cudaSuccess) e = cudaDeviceSynchronize();
-        if (e == cudaSuccess) e = cudaHostAlloc(reinterpret_cast<void**>(&h->error), sizeof(int), cudaHostAllocMapped);
-        if (e == cudaSuccess) *h->error = 0;
+        if (e == cudaSuccess) e = error_words().take(&h->error);
         if (e != cudaSuccess) {
             cudaGetLastError();
-            moe_kv4_destroy(h);
             return report_error(e == cudaErrorMemoryAllocation ? MOE_ERR_OOM : MOE_ERR_CUDA,
                                 std::string("moe_kv4_create: ") + cudaGetErrorString(e));
         }
         h->bytes = part + counter;
-        *out = h;
+        *out = h.release();
         return MOE_OK;
     });
 }
@@ -1299,9 +1345,8 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
 void moe_kv4_destroy(MoeKv4* h) {
     if (!h) return;
     OnDevice on(h->cfg.device);
-    cudaFree(h->part);
-    cudaFree(h->counter);
-    cudaFreeHost(h->error);
+    cudaFree(h->part);     // waits for what still uses it
+    error_words().give(h->error);
     delete h;
 }
 

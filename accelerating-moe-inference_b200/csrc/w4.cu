@@ -742,12 +742,12 @@ using namespace moe;
 struct MoeW4 {
     MoeW4Config cfg;
     int outputs = 0, tiles = 0, blocks = 0, sms = 0;
-    uint8_t* records = nullptr;
+    uint8_t* records = nullptr;   // with the first workspaces behind them
     Planes x{};               // the activations' operand, of work_rows rows
     float* result = nullptr;  // fp32 results of the experts, result_size values
     size_t result_size = 0;
     int work_rows = 0;
-    std::vector<void*> held;  // the workspaces, outgrown ones too: enqueued work and graphs name them
+    std::vector<void*> held;  // further workspaces, outgrown ones too: enqueued work and graphs name them
     size_t bytes = 0;
 };
 
@@ -776,22 +776,35 @@ int hold(MoeW4* h, size_t bytes, cudaStream_t s, uint8_t** out) {
     return MOE_OK;
 }
 
-// Operands for `rows` products; a handle that outgrows its own at least doubles
-// them, so that what it holds stays below twice the last.
+// Bytes of the operands of `rows` products: planes, sums, units.  Column tiles:
+// two columns a product, one not full for each matrix in use, and one that the
+// last pass of a kernel of two column tiles may look at.
+struct OperandBytes {
+    size_t plane, sums, unit;
+    OperandBytes(const MoeW4* h, int rows) {
+        const size_t tiles = rows ? (size_t)(2 * rows + 7) / 8 + std::min(rows, h->cfg.num_matrices) + 1 : 0;
+        plane = tiles * h->blocks * 2048;
+        sums = tiles * h->blocks * (kBlockK / h->cfg.group) * 8 * sizeof(float);
+        unit = ((size_t)rows * sizeof(float) + 255) / 256 * 256;
+    }
+    size_t all() const { return plane + sums + unit; }
+};
+
+void place_operands(MoeW4* h, int rows, uint8_t* at) {
+    const OperandBytes b(h, rows);
+    h->x = Planes{reinterpret_cast<uint4*>(at), reinterpret_cast<float*>(at + b.plane), reinterpret_cast<float*>(at + b.plane + b.sums)};
+    h->work_rows = rows;
+}
+
+// A handle that outgrows its operands at least doubles them, so that what it
+// holds stays below twice the last.
 int ensure_rows(MoeW4* h, int rows, cudaStream_t s) {
     if (rows <= h->work_rows) return MOE_OK;
     rows = std::max(rows, std::min(2 * h->work_rows, kMaxRows));
-    // Column tiles: two columns a product, one not full for each matrix in use,
-    // and one that the last pass of a kernel of two column tiles may look at.
-    const size_t tiles = (size_t)(2 * rows + 7) / 8 + std::min(rows, h->cfg.num_matrices) + 1;
-    const size_t plane = tiles * h->blocks * 2048, unit = rows * sizeof(float);
-    const size_t sums = tiles * h->blocks * (kBlockK / h->cfg.group) * 8 * sizeof(float);   // a multiple of 32
     uint8_t* at = nullptr;
-    const int rc = hold(h, plane + sums + unit, s, &at);
-    if (rc != MOE_OK) return rc;
-    h->x = Planes{reinterpret_cast<uint4*>(at), reinterpret_cast<float*>(at + plane), reinterpret_cast<float*>(at + plane + sums)};
-    h->work_rows = rows;
-    return MOE_OK;
+    const int rc = hold(h, OperandBytes(h, rows).all(), s, &at);
+    if (rc == MOE_OK) place_operands(h, rows, at);
+    return rc;
 }
 
 // Lets the kernels that make operands for themselves have kInlineMax bytes.
@@ -809,10 +822,12 @@ template <int kPer> cudaError_t inline_attributes_all() {
     return e;
 }
 
-// Room for the experts' fp32 results of `rows` products: two parts where the
-// product may be split (launch_product), which is the down product.
+// Room for the experts' fp32 results of a product: two parts where it may be
+// split (launch_product), which is the down product.
+size_t result_row(const MoeW4* h) { return (size_t)h->outputs * (h->cfg.gated ? 1 : 2); }
+
 int ensure_result(MoeW4* h, int rows, cudaStream_t s) {
-    const size_t row = (size_t)h->outputs * (h->cfg.gated ? 1 : 2);
+    const size_t row = result_row(h);
     if (rows * row <= h->result_size) return MOE_OK;
     const size_t n = std::max(rows * row, std::min(2 * h->result_size, kMaxRows * row));
     uint8_t* at = nullptr;
@@ -860,13 +875,20 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     h->blocks = (cfg->cols + kBlockK - 1) / kBlockK;
     const int per = kBlockK / cfg->group, groups = (cfg->cols + cfg->group - 1) / cfg->group;
     const size_t matrix = (size_t)h->tiles * h->blocks * w4_record(per), E = cfg->num_matrices;
-    e = cudaMalloc(&h->records, matrix * E);
+    // One allocation (they are most of what a handle costs to make) for the records, the operands and
+    // the experts' results; a matrix that is neither gated nor one of several is not asked for those.
+    const size_t records = (matrix * E + 255) / 256 * 256, operands = OperandBytes(h, cfg->max_rows).all();
+    if (cfg->gated || cfg->num_matrices > 1) h->result_size = cfg->max_rows * result_row(h);
+    h->bytes = records + operands + h->result_size * sizeof(float);
+    e = cudaMalloc(&h->records, h->bytes);
     if (e != cudaSuccess) {
         cudaGetLastError();
         delete h;
-        return report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed");
+        return e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed")
+                                              : launch_status(e, "moe_w4_create");
     }
-    h->bytes = matrix * E;
+    place_operands(h, cfg->max_rows, h->records + records);
+    h->result = reinterpret_cast<float*>(h->records + records + operands);
     // Host weights pass through the device one matrix at a time.
     const size_t nc = (size_t)cfg->rows * (cfg->cols / 2), ng = (size_t)cfg->rows * groups;
     uint8_t* stage = nullptr;
@@ -889,11 +911,8 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     }
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     cudaFree(stage);
-    int rc = e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed")
-                                            : launch_status(e, "moe_w4_create");
-    if (rc == MOE_OK) rc = ensure_rows(h, cfg->max_rows, nullptr);
-    // The experts' matrices; others are not asked for results of that kind.
-    if (rc == MOE_OK && (cfg->gated || cfg->num_matrices > 1)) rc = ensure_result(h, cfg->max_rows, nullptr);
+    const int rc = e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed")
+                                                  : launch_status(e, "moe_w4_create");
     if (rc != MOE_OK) {
         cudaGetLastError();
         moe_w4_destroy(h);

@@ -47,3 +47,27 @@ def test_a_small_handle_beside_a_large_one(R):
             plan_once(large, cached, new, bs, W, R * W, R)
             plan_once(small, cached[:1], new[:1], bs, W, 4, 1)
         plan_once(large, cached, new, bs, W, R * W, R)
+
+
+@pytest.mark.gpu
+def test_many_handles_alive():
+    """More handles than share a page of pinned memory, each with a workspace and
+    an error word of its own; what is destroyed serves the next ones."""
+    import torch
+    from test_kv4 import Batch
+    pkg = load_pkg()
+    b = Batch(pkg, [100, 7], [1, 1], H=2, Hkv=1, D=64, bs=16, dt=0)
+    want, lse = b.run()
+    first = b.kv
+    kw = dict(num_kv_heads=1, head_dim=64, block_tokens=16, num_blocks=b.nb, table_width=b.W,
+              max_requests=2)
+    for _ in range(2):
+        many = [pkg.Kv4Cache(**kw) for _ in range(1030)]
+        for h in (many[0], many[512], many[-1]):
+            b.kv = h
+            out, ls = b.run()
+            assert torch.equal(out, want) and torch.equal(ls, lse)
+        for h in many:
+            h.close()
+    b.kv = first
+    assert torch.equal(b.run()[0], want)
