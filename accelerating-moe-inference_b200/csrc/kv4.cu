@@ -174,8 +174,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
             copy(take, [&](int i) { return a.ring[wrap((long long)head + f + i)]; }, [&](int i, int v) { row[used + i] = v; });
         }
     }
-    // The tokens: a thread each.
-    for (int t = blockIdx.x * kPlanThreads + threadIdx.x; t < a.cap; t += gridDim.x * kPlanThreads) {
+    // The tokens: a thread each.  Unsigned: the last step may pass 2^31.
+    for (unsigned at = blockIdx.x * kPlanThreads + threadIdx.x; at < (unsigned)a.cap; at += gridDim.x * kPlanThreads) {
+        const int t = (int)at;
         int pos = -1;
         long long slot = -1;
         if (t < q_off[a.R]) {

@@ -71,3 +71,34 @@ def test_many_handles_alive():
             h.close()
     b.kv = first
     assert torch.equal(b.run()[0], want)
+
+
+@pytest.mark.gpu
+def test_plan_with_the_largest_token_count():
+    """A step of 2^31 - 1 places, of which three requests use a few (26 GB of
+    outputs): every place is written once, none beyond."""
+    import torch
+    pkg = load_pkg()
+    cap, bs, W, nb = 2 ** 31 - 1, 16, 8, 16
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    cached, new = i32(3, 16, 0), i32(20, 1, 5)
+    ring, state = torch.arange(nb, dtype=torch.int32, device="cuda"), i32(0, nb)
+    table = torch.full((3, W), -1, dtype=torch.int32, device="cuda")
+    table[0, 0], table[1, 0] = 14, 15
+    kv_len, q_offset, out = i32(0, 0, 0), i32(0, 0, 0, 0), i32(0, 0)
+    pad = 1024
+    pos = torch.full((cap + pad,), -7, dtype=torch.int32, device="cuda")
+    slot = torch.full((cap + pad,), -7, dtype=torch.int64, device="cuda")
+    with pkg.Kv4Cache(num_kv_heads=1, head_dim=64, block_tokens=bs, num_blocks=nb, table_width=W,
+                      max_requests=3) as kv:
+        kv.plan(cached.data_ptr(), new.data_ptr(), 3, ring.data_ptr(), state.data_ptr(),
+                table.data_ptr(), kv_len.data_ptr(), q_offset.data_ptr(), pos.data_ptr(),
+                slot.data_ptr(), cap, out.data_ptr(), stream())
+        torch.cuda.synchronize()
+    assert q_offset.tolist() == [0, 20, 21, 26] and kv_len.tolist() == [23, 17, 5]
+    assert pos[:26].tolist() == [*range(3, 23), 16, *range(5)]
+    # One new page each: 0, 1 and 2 of the ring.
+    assert slot[:26].tolist() == [*range(14 * 16 + 3, 15 * 16), *range(7), 16, *range(32, 37)]
+    for x in (pos, slot):
+        assert all((x[a:min(a + (1 << 28), cap)] == -1).all() for a in range(26, cap, 1 << 28))
+        assert (x[cap:] == -7).all()
