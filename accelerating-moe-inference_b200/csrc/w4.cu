@@ -249,6 +249,12 @@ template <class T> __device__ __forceinline__ void load_chunk(const T* row, int 
     }
 }
 
+// The lanes of chunk c's warp whose chunks a row of `chunks` has, where lanes
+// hold neighbouring chunks: chunks is a multiple of 16, so all or the lower half.
+__device__ __forceinline__ unsigned chunk_lanes(int c, int chunks) {
+    return chunks - (c & ~31) >= 32 ? 0xffffffffu : 0xffffu;
+}
+
 __device__ __forceinline__ float chunk_max(const float (&v)[8]) {
     float m = 0.0f;
 #pragma unroll
@@ -318,11 +324,11 @@ template <class T, int kPlanes> __global__ void __launch_bounds__(1024) w4_plane
     const RowScale scale(mx);
     if (threadIdx.x == 0) a.out.unit[row] = scale.unit;
     const int first = row * a.share, last = min(a.num_rows, first + a.share);
-    auto put = [&](int c, float (&v)[8]) {     // chunks is a multiple of 16: whole groups of lanes
+    auto put = [&](int c, float (&v)[8]) {     // by all of chunk_lanes(): whole groups of lanes
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += v[i] *= scale.up;
-        const unsigned live = __activemask();
+        const unsigned live = chunk_lanes(c, chunks);
         for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
         uint4 b[kPlanes];
         operands<kPlanes>(v, b);
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
 #pragma unroll
                 for (int k = 0; k < kPlanes; ++k) inline_x[(c / 4 * columns + t * kPlanes + k) * 4 + c % 4] = b[k];
                 if constexpr (kPlanes == 1) {
-                    const unsigned live = __activemask();
+                    const unsigned live = chunk_lanes(c, chunks);
 #pragma unroll
                     for (int o = 1; o < kChunks; o <<= 1) sum += __shfl_xor_sync(live, sum, o);
                     if (c % kChunks == 0) sums[c / kChunks * 8 + t] = sum * (1.0f / 1048576.0f);
