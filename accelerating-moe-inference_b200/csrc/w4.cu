@@ -697,12 +697,12 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
         for (int i = threadIdx.x; i < out_rows * now; i += kThreads) {
             const int r = i % out_rows, token = i / out_rows;
             const int product = rows[t0 + token];
-            const float unit = (kInline ? units[token] : __ldg(a.x.unit + a.x_share.div(product))) * (kPlanes == 2 ? 1024.0f : 1048576.0f);
+            const float unit = kInline ? units[token] : __ldg(a.x.unit + a.x_share.div(product));
             auto total = [&](int row) {
                 float v = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kWarps; ++k) v += part[k][row][token];
-                return v * unit;
+                return v * (kPlanes == 2 ? 1024.0f : 1048576.0f) * unit;   // unit times the power may pass 2^127
             };
             float v;
             int out;
