@@ -961,7 +961,7 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     using Plane = std::conditional_t<kPlanes == 2, float, __half>;   // made apart, only the planes count
     const MoeW4Config& c = h->cfg;
-    const int x_rows = (num_rows + x_share - 1) / x_share;
+    const int x_rows = (num_rows - 1) / x_share + 1;   // num_rows > 0; x_share may be the largest integer
     const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1,
                        aligned16(x) && x_stride * (int64_t)sizeof(T) % 16 == 0};
     const MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,

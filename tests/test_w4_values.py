@@ -34,3 +34,18 @@ def test_rows_near_the_ends_of_a_type(dt, size, rows, K, group):
     assert (got[:, 5] == 0).all()
     tol = product_bound(d, xd, dt, want) + (2.0 ** -126 if size < 1 else 0)   # subnormal results may be flushed
     assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,K,N", [(2, 128, 40), (17, 192, 40), (9, 4096, 1100)])
+def test_one_row_of_x_for_all_products(rows, K, N, dt):
+    """x_share up to the largest integer."""
+    pkg = load_pkg()
+    w = weights(7, 1, N, K, 64, True)
+    x = on_gpu(np.random.default_rng(0).standard_normal((1, K)), dt)
+    d, xd = dense(*w, 64)[0], x.double().cpu().numpy()
+    want = (xd @ d.T).repeat(rows, 0)
+    for share in (rows, 2 ** 31 - 1):
+        got = product(pkg, w, x.expand(rows, K), dt, 64, x_share=share)
+        assert (np.abs(got - want) <= product_bound(d, xd, dt, want)).all()
