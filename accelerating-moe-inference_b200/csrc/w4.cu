@@ -229,6 +229,7 @@ struct PlanesArgs {
     Planes out;
     int cols, blocks, group, num_rows, share, E;
     bool vec;              // rows of x can be read 16 bytes at a time
+    int dtype;             // of x
 };
 
 // Eight inputs of a row from `k` on, zeros past its end.
@@ -263,13 +264,14 @@ __device__ __forceinline__ float chunk_max(const float (&v)[8]) {
 }
 
 // Exponent of a row's largest, kept where 2^(10 - e) is a normal number, the
-// factor 2^(10 - e) that scales the row and its inverse.
+// factor 2^(10 - e) that scales the row and its inverse.  A row that holds an
+// infinity has an infinite unit (see defined_product).
 struct RowScale {
     float up, unit;
     __device__ explicit RowScale(float largest) {
         const int e = min(max((int)(__float_as_uint(largest) >> 23), 11), 253);
         up = __uint_as_float((264 - e) << 23);
-        unit = __uint_as_float((e - 10) << 23);
+        unit = isinf(largest) ? largest : __uint_as_float((e - 10) << 23);
     }
 };
 
@@ -381,6 +383,39 @@ __device__ __forceinline__ void store_as(void* y, long long at, float v, int dty
     else static_cast<__half*>(y)[at] = from_f32<__half>(v);
 }
 
+// Rows of x that hold an infinity.  Codes that are counted from their zeros only
+// behind the sum, or planes whose second holds what the first leaves, would make
+// NaN where an infinity of the weight's sign is due, so such a row's products are
+// made by the definition, term by term: slow, and apart from the hot loop.
+__device__ __noinline__ float load_as(const void* x, int dtype, int k) {
+    return dtype == MOE_DTYPE_F32    ? static_cast<const float*>(x)[k]
+           : dtype == MOE_DTYPE_BF16 ? to_f32(static_cast<const __nv_bfloat16*>(x)[k])
+                                     : to_f32(static_cast<const __half*>(x)[k]);
+}
+
+__device__ __noinline__ bool has_infinity(const void* x, int dtype, int cols) {
+    for (int k = 0; k < cols; ++k)
+        if (isinf(load_as(x, dtype, k))) return true;
+    return false;
+}
+
+// Over the blocks of 128 columns [kb, kb_end); `rec` is the record of the weight
+// row's tile at column block 0, `row` its row.
+template <int kPer>
+__device__ __noinline__ float defined_product(const uint8_t* rec, int row, int kb, int kb_end, const void* x, int dtype, int cols) {
+    float sum = 0.0f;
+    for (; kb < kb_end; ++kb) {
+        const uint8_t* at = rec + (long long)kb * (4 * w4_record(kPer));
+        for (int i = 0; i < kBlockK / 8 && kb * kBlockK + i * 8 < cols; ++i) {      // word i / 4 of lane 4 (row % 8) + i % 4
+            const uint32_t word = reinterpret_cast<const uint32_t*>(at)[(row / 8 * 32 + row % 8 * 4 + i % 4) * 4 + i / 4];
+            const float2 p = __half22float2(reinterpret_cast<const __half2*>(at + 1024)[(row % 8 * 2 + row / 8) * kPer + i * kPer / 16]);
+            for (int n = 0; n < 8; ++n)
+                sum = fmaf(p.x * ((float)(word >> (4 * n) & 15) - p.y), load_as(x, dtype, kb * kBlockK + i * 8 + n), sum);
+        }
+    }
+    return sum;
+}
+
 // y = W x.  An item is (matrix in use, part of the columns, MT tiles of 16
 // weight rows); the thread blocks take the items in turn, a warp every
 // kWarps-th block of 128 columns.  One part is all columns; two, for results
@@ -421,8 +456,10 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
     __shared__ Sorted sorted;
     __shared__ float units[8];
     __shared__ int largest[8];
+    __shared__ bool infinite;           // a row of x that the block has seen holds an infinity
     extern __shared__ __align__(16) uint4 inline_x[];   // [block * 4 + w][column][4 j], then the sums
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+    if (threadIdx.x == 0) infinite = false;
     sort_products<kThreads, kPlanes>(sorted, a.matrix, a.num_rows, a.E);
     const int items = sorted.used * a.groups.d;
 
@@ -698,6 +735,7 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
             const int r = i % out_rows, token = i / out_rows;
             const int product = rows[t0 + token];
             const float unit = kInline ? units[token] : __ldg(a.x.unit + a.x_share.div(product));
+            if (isinf(unit)) infinite = true;
             auto total = [&](int row) {
                 float v = 0.0f;
 #pragma unroll
@@ -719,6 +757,39 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
         }
         item = next;
         t0 = next_t0;
+    }
+
+    // The products of rows that hold an infinity once more, in place of what the
+    // operands gave for them.
+    __syncthreads();
+    if (!infinite) return;
+    const int x_bytes = xa.dtype == MOE_DTYPE_F32 ? 4 : 2, out_rows = a.gated ? MT * 8 : MT * 16;
+    for (item = blockIdx.x; item < items; item += gridDim.x) {
+        const auto [m, tile, part_of] = place_of(item);
+        const short* rows = sorted.rows + sorted.first[m];
+        const int n = sorted.first[m + 1] - sorted.first[m];
+        for (int i = threadIdx.x; i < out_rows * n; i += kThreads) {
+            const int r = i % out_rows, product = rows[i / out_rows], x_row = a.x_share.div(product);
+            const uint8_t* x = static_cast<const uint8_t*>(xa.x) + x_row * xa.stride * x_bytes;
+            if (!(kInline ? has_infinity(x, xa.dtype, xa.cols) : isinf(__ldg(a.x.unit + x_row)))) continue;
+            auto total = [&](int row) {
+                const int t = tile + row / 16;
+                const uint8_t* rec = a.records + ((long long)sorted.matrix[m] * (a.tiles / 4) + t / 4) * a.blocks * (4 * kRecord) + t % 4 * kRecord;
+                return defined_product<kPer>(rec, row % 16, part_of * a.blocks_part, min(a.blocks, (part_of + 1) * a.blocks_part), x,
+                                             xa.dtype, xa.cols);
+            };
+            float v;
+            int out;
+            if (a.gated) {
+                v = total(r / 16 * 32 + r % 16);
+                v = v / (1.0f + expf(-v)) * total(r / 16 * 32 + 16 + r % 16);
+                out = (tile / 2 + r / 16) * 16 + r % 16;
+            } else {
+                v = total(r);
+                out = tile * 16 + r;
+            }
+            if (out < a.outputs) store_as(a.y, ((long long)part_of * a.num_rows + product) * a.outputs + out, v, a.dtype);
+        }
     }
 }
 
@@ -961,9 +1032,10 @@ cudaError_t product(const MoeW4* h, const T* x, int num_rows, int64_t x_stride, 
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
     using Plane = std::conditional_t<kPlanes == 2, float, __half>;   // made apart, only the planes count
     const MoeW4Config& c = h->cfg;
+    constexpr int x_dtype = kPlanes == 2 ? MOE_DTYPE_F32 : std::is_same_v<T, __half> ? MOE_DTYPE_F16 : MOE_DTYPE_BF16;
     const int x_rows = (num_rows - 1) / x_share + 1;   // num_rows > 0; x_share may be the largest integer
     const PlanesArgs p{x, x_stride, matrix, h->x, c.cols, h->blocks, c.group, num_rows, x_share, matrix ? c.num_matrices : 1,
-                       aligned16(x) && x_stride * (int64_t)sizeof(T) % 16 == 0};
+                       aligned16(x) && x_stride * (int64_t)sizeof(T) % 16 == 0, x_dtype};
     const MatvecArgs a{h->records, h->x, matrix, y, num_rows, matrix ? c.num_matrices : 1, h->tiles, h->blocks, h->outputs, dtype,
                        FastDiv(x_share), FastDiv(), c.gated != 0, (h->outputs + 15) / 16 * (c.gated ? 2 : 1), 0, 0};
     const int used = matrix ? std::min(num_rows, c.num_matrices) : 1;

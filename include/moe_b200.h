@@ -674,7 +674,9 @@ size_t moe_w4_device_bytes(const MoeW4* h);
  * may be null: matrix 0): the matrix of each product; a row whose entry is
  * outside [0, num_matrices) gets zeros.  Sums are in fp32; x enters the
  * products as float16 scaled by a power of two per row: 16-bit types exactly
- * (to 2^-34 of the row's largest), fp32 with 22 significant bits. */
+ * (to 2^-34 of the row's largest), fp32 with 22 significant bits.  A row that
+ * holds an infinity or a NaN gives what the sum over its terms gives (slowly
+ * for an infinity); other rows do not change. */
 int moe_w4_matvec_device(MoeW4* h, const void* x, int32_t dtype, int32_t num_rows,
                          int64_t x_row_stride, int32_t x_share, const int32_t* matrix, void* y,
                          void* stream);
