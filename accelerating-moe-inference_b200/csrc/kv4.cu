@@ -561,7 +561,10 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 //   q . k = s (q . c) + m sum(q),
 // those of a value go into the probabilities before the second product,
 //   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t m_t.
-// fp32: with c - 8 in the place of c and m + 8 s in that of m.
+// Keys, and values for fp32 results: with c - 8 in the place of c and m + 8 s in
+// that of m (see codes(); with keys as subnormals the lse of one key was off by
+// 1.1e-6 for float16 queries, six times as far as plain fp32, and attend_long
+// took 112 us instead of 118; with values as normal numbers too it takes 124).
 // Two planes: fp32 queries, and any type's p s, enter as two float16 numbers, hi
 // and (x - hi) 2^11, in neighbouring columns of the same product (22 bits).
 // 16-bit types take them where up to four rows leave the columns free, which
@@ -587,8 +590,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     constexpr int kPitch = D + 4;              // floats per output row in shared memory
     constexpr int kThreads = kAttendWarps * 32;
     constexpr float kLo = 1.0f / 2048.0f;      // weight of the low plane
-    constexpr bool kNormal = sizeof(T) == 4;   // fp32 results need the whole of their sums
-    constexpr float kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
+    // Scores are fp32 whatever the type, and lse shows them; of the values' sums
+    // fp32 results need the whole.
+    constexpr bool kNormal = sizeof(T) == 4;
+    constexpr float kKeyUnit = 64.0f, kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
     constexpr float kCentre = kNormal ? 8.0f : kPlanes == 1 ? 7.5f : 0.0f;   // the code that values are counted from
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     constexpr int kStage = 2 * kGran;
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             // Exponent of the largest, kept where 2^(10 - e) is a normal number.
             const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
             const float up = copysignf(__uint_as_float((264 - e) << 23), a.scale);   // +-2^(10 - (e - 127))
-            const float f = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kUnit, 1e-37f);
+            const float f = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kKeyUnit, 1e-37f);
             float sum[G];
 #pragma unroll
             for (int q = 0; q < G; ++q) {
@@ -771,7 +776,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                     for (int k = 0; k < 8; ++k) sum[q] += x[w][k] *= up;
                 sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], 1);
                 sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], 2);
-                sum[q] *= 1.0f / kUnit;
+                sum[q] *= 1.0f / kKeyUnit;
             }
 #pragma unroll
             for (int w = 0; w < 2 * G; ++w)
@@ -857,8 +862,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                         for (int k = 0; k < 2; ++k) {
                             const int w = 2 * q + (step >> 1), shift = 8 * (step & 1);
                             const uint32_t lo = kw[k][0][w] >> shift, hi = kw[k][1][w] >> shift;
-                            const uint32_t f[4] = {codes<kNormal>(lo, kEven), codes<kNormal>(hi, kEven),
-                                                   codes<kNormal>(lo, kOdd), codes<kNormal>(hi, kOdd)};
+                            const uint32_t f[4] = {codes<true>(lo, kEven), codes<true>(hi, kEven),
+                                                   codes<true>(lo, kOdd), codes<true>(hi, kOdd)};
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 const uint32_t(&b)[2] = qb[n][2 * w + (step & 1)];
@@ -886,7 +891,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                                 const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
                                 const float (&t)[4] = acc[k][i / kE][q];
                                 const float d = kPlanes == 2 ? fmaf(t[2 * h + 1], kLo, t[2 * h]) : t[2 * h + i % kE];
-                                const float zero = kNormal ? fmaf(p.x, 8.0f, p.y) : p.y;
+                                const float zero = fmaf(p.x, 8.0f, p.y);
                                 s = q == 0 ? zero * qs[i][q] : fmaf(zero, qs[i][q], s);
                                 s = fmaf(p.x, d, s);
                             }

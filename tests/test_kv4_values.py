@@ -220,3 +220,23 @@ def test_16_bit_results_are_as_good_as_their_type(H, Hkv, nq, dt):
     most = 1.5 if dt == 1 or H // Hkv * nq <= 4 else (1 + 1.5 ** 2) ** 0.5
     err = (out.double() - want).norm().item()
     assert err <= most * once, (err / once, most)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H", [4, 8, 24])
+@pytest.mark.parametrize("dt", [0, 1, 2], ids=["f32", "bf16", "f16"])
+def test_lse_of_one_key(dt, H, D):
+    """The log of the sum is fp32 whatever the type, and of one key it is the
+    score.  A score of unit size is a sum of D / 16 steps whose partial sums are of
+    that size too, each off by an error spread over 2^-23 of it: together sqrt(8 /
+    3) 2^-23 at D = 128.  Twice that and more, with the exponential's and the
+    logarithm's: 2^-21 of the norm."""
+    lens = (1,) * 96
+    b = batch(dt, D, H=H, Hkv=4, lens=lens, nqs=lens)
+    k, v = keys_and_values(b)
+    refill(b, k, v)
+    _, ls = b.run()
+    _, want, *_ = exact(b)
+    err = (ls.double() - want).norm().item()
+    assert err <= 2.0 ** -21 * want.norm().item(), err / want.norm().item()
