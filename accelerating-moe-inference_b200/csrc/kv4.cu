@@ -335,10 +335,12 @@ __device__ __forceinline__ uint32_t quantise8(float2 (&x)[4], __half2& param) {
 // shuffles.  A granule's codes lie in pieces of 4 to 16 bytes per token, so 16
 // tokens that fill a granule (a prompt's, from a multiple of 16 on) are put
 // together in shared memory and written as whole lines; others (a decode
-// step's) are written piece by piece.  Bound by its instructions, about 25 a
-// value, most of them the quantiser's, hence the pairwise fp32 operations:
-// 49 us for 16384 tokens x 8 heads x 128 of bf16 with the values written back,
-// 153 MB at 3.1 TB/s (a thread per 8 dims of K or V, with divisions: 86 us).
+// step's) are written piece by piece.  A block loads, quantises and stores once,
+// so that nothing of its own runs beneath its loads: waiting for them is by far
+// the largest stall (4.7 cycles an instruction), 2.5 of 4 instructions are issued
+// a cycle, about 25 a value, hence the pairwise fp32 operations.  49 to 50 us for
+// 16384 tokens x 8 heads x 128 of bf16 with the values written back, 153 MB at
+// 3.1 TB/s (a thread per 8 dims of K or V, with divisions: 86 us).
 template <class T, int D, bool kVec> __global__ void __launch_bounds__(D, 1024 / D) append_kernel(AppendArgs a) {
     constexpr int G = D / 64, kThreads = D, kGran = kv4_granule(D);   // D / 8 threads per token
     __shared__ __align__(16) uint8_t stage[kGran];
@@ -555,8 +557,8 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // probabilities of 16 tokens x 8 rows become the second product's B by an 8x8
 // transposition between the lanes.  A 4-bit code in the low bits of a float16
 // word is the subnormal c 2^-24 (or c 2^-20 four bits higher), so a code pair
-// becomes an operand by one AND, exactly (fp32: by one AND and one
-// multiplication, see codes()).  The scale and minimum of a key stand outside
+// becomes an operand by one AND, exactly (a normal number by one fma more, see
+// codes()).  The scale and minimum of a key stand outside
 // its product,
 //   q . k = s (q . c) + m sum(q),
 // those of a value go into the probabilities before the second product,
@@ -575,10 +577,13 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 // (float16 results of 8 rows and 100 to 2048 keys: 1.13 times what their own
 // rounding leaves instead of 1.75, at no cost that shows).
 //
-// Bound by its instructions, about 270 a granule of 2304 bytes at two a cycle.
-// 8 requests of 16 k to 131 k tokens, 32 query and 8 key/value heads of 128,
-// f16: 112 to 122 us, 509 MB at 4.2 to 4.5 TB/s (the copies alone: 85 us); 64
-// requests of 100 to 8192, bf16: 47 us; one of 640, 16 heads, fp32: 12 us.
+// Bound by the serial chain of a pair of granules (products, maximum,
+// exponentials, products) on the 12 warps an SM that registers and the rings
+// leave: about 330 instructions a granule of 2304 bytes, 2.2 of 4 issued a cycle
+// with 2.8 warps a scheduler, most stalls on the instruction before.  8 requests
+// of 16 k to 131 k tokens, 32 query and 8 key/value heads of 128, f16: 118 us (120
+// in a long run), 509 MB at 4.3 TB/s (the copies alone: 85 us); 64 requests of
+// 100 to 8192, bf16: 47.5 us; one of 640, 16 heads, fp32: 12 us.
 // NT: column tiles of 8; two take 16 query rows (fp32: 8) per unpacking.
 template <class T, int D, int NT, int kPlanes>
 __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm : 2) attend_kernel(AttendArgs a) {

@@ -433,11 +433,15 @@ __device__ __noinline__ float defined_product(const uint8_t* rec, int row, int k
 // normal number (c - z) 2^-10 by one fma.  The warps' sums are added in order
 // through shared memory.
 //
-// Measured: 8 experts' gate/up (28672 x 4096 each, 16 products, bf16) 89 us,
-// 499 MB at 5.6 TB/s, 81 instructions a record; their down products (4096 x
-// 14336, fp32) 57 us in one part, 3.46 turns of the blocks, and 51 in two.  16
-// rows of 32000 x 2048 (bf16) 18 us, bound by the warps that registers leave;
-// one of 2048 x 2048 (fp32) 6.2 us with its launch.
+// Measured: 8 experts' gate/up (28672 x 4096 each, 16 products, bf16) 88 us, 499
+// MB at 5.7 TB/s, 82 instructions a record; their down products (4096 x 14336,
+// fp32) 50 us in two parts (both products and the sum back to back: 140 us, 142
+// with one part, 3.46 turns of the blocks).  16 rows of 32000 x 2048 (bf16) 22.6
+// us with their operands' kernel: 4 records a warp between two joins, 16 warps an
+// SM, waiting for records most of the time; one row of 2048 x 2048 (fp32) 6.2 us
+// with its launch.  The launch bounds are what groups of 128 need; with groups of
+// 64 and 32, whose params take two and four times the registers, some variants
+// spill (up to 384 bytes, the one with four tiles and groups of 32).
 //
 // kInline: few activations (product() below) are made operands by every block
 // for itself, in shared memory, instead of by a kernel of their own; that saves
@@ -765,17 +769,17 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
     if (!infinite) return;
     const int x_bytes = xa.dtype == MOE_DTYPE_F32 ? 4 : 2, out_rows = a.gated ? MT * 8 : MT * 16;
     for (item = blockIdx.x; item < items; item += gridDim.x) {
-        const auto [m, tile, part_of] = place_of(item);
-        const short* rows = sorted.rows + sorted.first[m];
-        const int n = sorted.first[m + 1] - sorted.first[m];
+        const Place at = place_of(item);
+        const short* rows = sorted.rows + sorted.first[at.m];
+        const int n = sorted.first[at.m + 1] - sorted.first[at.m];
         for (int i = threadIdx.x; i < out_rows * n; i += kThreads) {
             const int r = i % out_rows, product = rows[i / out_rows], x_row = a.x_share.div(product);
             const uint8_t* x = static_cast<const uint8_t*>(xa.x) + x_row * xa.stride * x_bytes;
             if (!(kInline ? has_infinity(x, xa.dtype, xa.cols) : isinf(__ldg(a.x.unit + x_row)))) continue;
             auto total = [&](int row) {
-                const int t = tile + row / 16;
-                const uint8_t* rec = a.records + ((long long)sorted.matrix[m] * (a.tiles / 4) + t / 4) * a.blocks * (4 * kRecord) + t % 4 * kRecord;
-                return defined_product<kPer>(rec, row % 16, part_of * a.blocks_part, min(a.blocks, (part_of + 1) * a.blocks_part), x,
+                const int t = at.tile + row / 16;
+                const uint8_t* rec = a.records + ((long long)sorted.matrix[at.m] * (a.tiles / 4) + t / 4) * a.blocks * (4 * kRecord) + t % 4 * kRecord;
+                return defined_product<kPer>(rec, row % 16, at.part * a.blocks_part, min(a.blocks, (at.part + 1) * a.blocks_part), x,
                                              xa.dtype, xa.cols);
             };
             float v;
@@ -783,12 +787,12 @@ __global__ void __launch_bounds__(w4_threads(NT), w4_blocks(MT, NT)) w4_matvec_k
             if (a.gated) {
                 v = total(r / 16 * 32 + r % 16);
                 v = v / (1.0f + expf(-v)) * total(r / 16 * 32 + 16 + r % 16);
-                out = (tile / 2 + r / 16) * 16 + r % 16;
+                out = (at.tile / 2 + r / 16) * 16 + r % 16;
             } else {
                 v = total(r);
-                out = tile * 16 + r;
+                out = at.tile * 16 + r;
             }
-            if (out < a.outputs) store_as(a.y, ((long long)part_of * a.num_rows + product) * a.outputs + out, v, a.dtype);
+            if (out < a.outputs) store_as(a.y, ((long long)at.part * a.num_rows + product) * a.outputs + out, v, a.dtype);
         }
     }
 }
