@@ -15,6 +15,11 @@ namespace moe {
 
 int report_error(int code, const std::string& msg);  // capi.cu
 
+// Memory of a handle on `device`, which is current; 1024-byte aligned.  handle_free
+// waits for the current device (handle_memory.cu).
+cudaError_t handle_alloc(int device, size_t bytes, void** out);
+void handle_free(void* p) noexcept;
+
 template <class T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -1335,7 +1335,7 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
         const size_t grid = (size_t)sms * kAttendCtasPerSm;
         const size_t part = grid * 2 * 16 * (cfg->head_dim + 2) * sizeof(float);
         const size_t counter = grid * sizeof(int);
-        e = cudaMalloc(&h->part, part + counter);
+        e = handle_alloc(cfg->device, part + counter, reinterpret_cast<void**>(&h->part));
         if (e == cudaSuccess) {
             h->counter = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(h->part) + part);
             e = cudaMemset(h->counter, 0, counter);
@@ -1356,7 +1356,7 @@ int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out) {
 void moe_kv4_destroy(MoeKv4* h) {
     if (!h) return;
     OnDevice on(h->cfg.device);
-    cudaFree(h->part);     // waits for what still uses it
+    handle_free(h->part);     // waits for what still uses it
     error_words().give(h->error);
     delete h;
 }

@@ -1,7 +1,7 @@
 // Matrix-vector products with 4-bit group-scaled weights, and the routed
 // experts built on them.
 #include <algorithm>
-#include <cstring>
+#include <memory>
 #include <type_traits>
 #include <new>
 #include <vector>
@@ -845,7 +845,7 @@ int hold(MoeW4* h, size_t bytes, cudaStream_t s, uint8_t** out) {
                                                  "call of this size before the capture");
     h->held.reserve(h->held.size() + 1);
     void* p = nullptr;
-    const cudaError_t e = cudaMalloc(&p, bytes);
+    const cudaError_t e = handle_alloc(h->cfg.device, bytes, &p);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "4-bit weights: workspace allocation failed")
@@ -947,7 +947,8 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     if (e != cudaSuccess) return launch_status(e, "moe_w4_create");
     if (!on.ok) return report_error(MOE_ERR_CUDA, "moe_w4_create: cannot select the device");
     if (major != 10) return report_error(MOE_ERR_UNSUPPORTED, "libmoe_b200 is built for sm_100a (B200) only");
-    auto* h = new MoeW4;
+    std::unique_ptr<MoeW4, void (*)(MoeW4*)> owner(new MoeW4, moe_w4_destroy);
+    MoeW4* h = owner.get();
     h->cfg = *cfg;
     h->sms = sms;
     h->outputs = cfg->gated ? cfg->rows / 2 : cfg->rows;
@@ -956,15 +957,14 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
     h->blocks = (cfg->cols + kBlockK - 1) / kBlockK;
     const int per = kBlockK / cfg->group, groups = (cfg->cols + cfg->group - 1) / cfg->group;
     const size_t matrix = (size_t)h->tiles * h->blocks * w4_record(per), E = cfg->num_matrices;
-    // One allocation (they are most of what a handle costs to make) for the records, the operands and
-    // the experts' results; a matrix that is neither gated nor one of several is not asked for those.
+    // One block for the records, the operands and the experts' results; a matrix that is neither
+    // gated nor one of several is not asked for those.
     const size_t records = (matrix * E + 255) / 256 * 256, operands = OperandBytes(h, cfg->max_rows).all();
     if (cfg->gated || cfg->num_matrices > 1) h->result_size = cfg->max_rows * result_row(h);
     h->bytes = records + operands + h->result_size * sizeof(float);
-    e = cudaMalloc(&h->records, h->bytes);
+    e = handle_alloc(cfg->device, h->bytes, reinterpret_cast<void**>(&h->records));
     if (e != cudaSuccess) {
         cudaGetLastError();
-        delete h;
         return e == cudaErrorMemoryAllocation ? report_error(MOE_ERR_OOM, "moe_w4_create: device allocation failed")
                                               : launch_status(e, "moe_w4_create");
     }
@@ -996,10 +996,9 @@ int w4_create(const MoeW4Config* cfg, const uint8_t* codes, const void* scales, 
                                                   : launch_status(e, "moe_w4_create");
     if (rc != MOE_OK) {
         cudaGetLastError();
-        moe_w4_destroy(h);
         return rc;
     }
-    *out = h;
+    *out = owner.release();
     return MOE_OK;
 }
 
@@ -1109,8 +1108,8 @@ int moe_w4_create_from_device(const MoeW4Config* cfg, const uint8_t* codes, cons
 void moe_w4_destroy(MoeW4* h) {
     if (!h) return;
     OnDevice on(h->cfg.device);
-    cudaFree(h->records);
-    for (void* p : h->held) cudaFree(p);
+    handle_free(h->records);
+    for (void* p : h->held) handle_free(p);
     delete h;
 }
 

@@ -540,9 +540,9 @@ typedef struct MoeKv4 MoeKv4;
  * positions and 16 requests, a pool that holds them all, device 0. */
 void moe_kv4_config_init(MoeKv4Config* cfg);
 /* The handle holds the geometry and the attention's workspace, no cache: one
- * handle serves every layer of a model.  One stream at a time.  Making one costs
- * a device allocation (0.35 ms, as much as hundreds of small calls on it): once
- * per model, not per step. */
+ * handle serves every layer of a model.  One stream at a time.  Its memory
+ * comes from slabs that handles of up to 64 MB share and the process keeps one
+ * of: making one costs 0.01 ms, where a new slab is due 0.5 to 2 ms. */
 int moe_kv4_create(const MoeKv4Config* cfg, MoeKv4** out);
 void moe_kv4_destroy(MoeKv4* h);
 /* Bytes of one cache buffer, and of the handle's workspace (0 for null). */
@@ -651,9 +651,10 @@ typedef struct MoeW4 MoeW4;
  * more allocates it; what it outgrows is freed with the handle only, so earlier
  * captures of the handle's calls stay good.  Such a call inside a stream
  * capture returns MOE_ERR_UNSUPPORTED and leaves the capture as it was.
- * Making a handle costs an allocation and a pass over the weights (0.35 ms for
- * 2048 x 2048, 1 ms for eight 28672 x 4096 that are on the device): for weights
- * that many calls use, not for one call's.
+ * Making a handle costs its memory (from shared slabs up to 64 MB, as for the
+ * cache's handles) and a pass over the weights: 0.02 ms for 2048 x 2048, 1 ms
+ * for eight 28672 x 4096 that are on the device.  For weights that many calls
+ * use, not for one call's.
  *
  * One matrix of 4096 x 4096, group 128, device 0, 16 product rows. */
 void moe_w4_config_init(MoeW4Config* cfg);

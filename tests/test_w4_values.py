@@ -143,3 +143,33 @@ def test_infinite_activations_experts(ff):
     # gate and up are infinities of either sign or NaN: silu gives inf, NaN at -inf;
     # some hidden values are NaN, so that every output is.
     assert torch.isnan(out[1][1]).all()
+
+
+@pytest.mark.gpu
+def test_handles_that_come_and_go():
+    """Handles of many sizes made and destroyed in turn: each keeps its weights and
+    its workspace to itself."""
+    import torch
+    pkg = load_pkg()
+    g = np.random.default_rng(11)
+    live = []
+    for step in range(60):
+        if len(live) > 12 or (live and g.random() < 0.35):
+            live.pop(int(g.integers(len(live))))[0].close()
+        N, K, group = int(g.integers(1, 900)), 32 * int(g.integers(1, 40)), int(g.choice([32, 64, 128]))
+        w = weights(step, 1, N, K, group, True)
+        live.append((pkg.W4Matrix(*w, group=group, max_rows=int(g.integers(0, 40))), w, group))
+        if step % 6:
+            continue
+        outs = []
+        for m, w, group in live:       # all at once: none waits for another's result
+            x = on_gpu(g.standard_normal((20, w[0].shape[2] * 2)), 0)
+            y = torch.full((20, w[0].shape[1]), -7, dtype=torch.float32, device="cuda")
+            m.matvec(x.data_ptr(), y.data_ptr(), 20, 0, stream())
+            outs.append((x, y))
+        for (m, w, group), (x, y) in zip(live, outs):
+            d, xd = dense(*w, group)[0], x.double().cpu().numpy()
+            want = xd @ d.T
+            assert (np.abs(y.double().cpu().numpy() - want) <= product_bound(d, xd, 0, want)).all()
+    for m, *_ in live:
+        m.close()
