@@ -441,7 +441,7 @@ __device__ __noinline__ float defined_product(const uint8_t* rec, int row, int k
 // SM, waiting for records most of the time; one row of 2048 x 2048 (fp32) 6.2 us
 // with its launch.  The launch bounds are what groups of 128 need; with groups of
 // 64 and 32, whose params take two and four times the registers, some variants
-// spill (up to 384 bytes, the one with four tiles and groups of 32).
+// spill (up to 412 bytes).
 //
 // kInline: few activations (product() below) are made operands by every block
 // for itself, in shared memory, instead of by a kernel of their own; that saves
