@@ -563,19 +563,22 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 //   q . k = s (q . c) + m sum(q),
 // those of a value go into the probabilities before the second product,
 //   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t m_t.
-// Keys, and values for fp32 results: with c - 8 in the place of c and m + 8 s in
-// that of m (see codes(); with keys as subnormals the lse of one key was off by
-// 1.1e-6 for float16 queries, six times as far as plain fp32, and attend_long
-// took 112 us instead of 118; with values as normal numbers too it takes 124).
+// fp32: with c - 8 in the place of c and m + 8 s in that of m (see codes()).
+// Scores are fp32 whatever the type, and lse shows them: of a code at c 2^-24 the
+// tensor core cuts off so much that the lse of one key was off by 1.1e-6 for
+// float16 queries, six times as far as plain fp32; keys' even nibbles are moved up
+// to c 2^-20 first (2.1e-7, attend_long 112 -> 118 us; normal numbers c - 8 for
+// every type did the same and cost 2 % more where a request has 8 rows).
 // Two planes: fp32 queries, and any type's p s, enter as two float16 numbers, hi
 // and (x - hi) 2^11, in neighbouring columns of the same product (22 bits).
 // 16-bit types take them where up to four rows leave the columns free, which
 // halves the softmax's work too (a lane has one row instead of two: attend_long
 // 118 us with one plane, 113 with two).  With one plane p s has 11 bits, and so
 // that its rounding counts on c - 7.5 only, not on c, a product with ones gives
-// the rounded numbers' sum: sum (p s)~ c - 7.5 sum (p s)~ + sum p (m + 7.5 s)
-// (float16 results of 8 rows and 100 to 2048 keys: 1.13 times what their own
-// rounding leaves instead of 1.75, at no cost that shows).
+// the rounded numbers' sum for float16 results: sum (p s)~ c - 7.5 sum (p s)~ +
+// sum p (m + 7.5 s) (8 rows and 100 to 2048 keys: 1.13 times what their own
+// rounding leaves instead of 1.75, for 3 % of the time; bfloat16 results, 1.01
+// times without it, go without).
 //
 // Bound by the serial chain of a pair of granules (products, maximum,
 // exponentials, products) on the 12 warps an SM that registers and the rings
@@ -595,11 +598,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     constexpr int kPitch = D + 4;              // floats per output row in shared memory
     constexpr int kThreads = kAttendWarps * 32;
     constexpr float kLo = 1.0f / 2048.0f;      // weight of the low plane
-    // Scores are fp32 whatever the type, and lse shows them; of the values' sums
-    // fp32 results need the whole.
-    constexpr bool kNormal = sizeof(T) == 4;
-    constexpr float kKeyUnit = 64.0f, kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
-    constexpr float kCentre = kNormal ? 8.0f : kPlanes == 1 ? 7.5f : 0.0f;   // the code that values are counted from
+    constexpr bool kNormal = sizeof(T) == 4;   // fp32 results need the whole of their sums
+    constexpr bool kOnesSum = kPlanes == 1 && std::is_same_v<T, __half>;   // bf16 results do not show it
+    constexpr float kUnit = kNormal ? 64.0f : 1048576.0f;   // what a code of an odd nibble is short of
+    constexpr float kCentre = kNormal ? 8.0f : kOnesSum ? 7.5f : 0.0f;   // the code that values are counted from
     constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
     constexpr int kStage = 2 * kGran;
     constexpr int kWarpFloats = kRows * kPitch + 2 * kRows;   // a warp's result
@@ -737,8 +739,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
     Segment sg;
     while (next_segment<kRows>(a, share, walk, sg)) {
         const int rows = sg.rows, tile = sg.tile, head = sg.head;
-        // The query fragments: rows scaled by a power of two to below 2^11,
-        // dims of even nibbles another 16 up to match their codes' 2^-24.
+        // The query fragments: rows scaled by a power of two to below 2^11, for
+        // fp32 the dims of even nibbles another 16 up, as their codes are 16 down.
         uint32_t qb[NT][D / 16][2];
         float qs[kR][G], rowf[kR];
         int row_pos[kR];
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
             // Exponent of the largest, kept where 2^(10 - e) is a normal number.
             const int e = min(max((int)(__float_as_uint(mx) >> 23), 11), 253);
             const float up = copysignf(__uint_as_float((264 - e) << 23), a.scale);   // +-2^(10 - (e - 127))
-            const float f = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kKeyUnit, 1e-37f);
+            const float f = fmaxf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((e - 10) << 23) * kUnit, 1e-37f);
             float sum[G];
 #pragma unroll
             for (int q = 0; q < G; ++q) {
@@ -781,13 +783,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                     for (int k = 0; k < 8; ++k) sum[q] += x[w][k] *= up;
                 sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], 1);
                 sum[q] += __shfl_xor_sync(0xffffffffu, sum[q], 2);
-                sum[q] *= 1.0f / kKeyUnit;
+                sum[q] *= 1.0f / kUnit;
             }
 #pragma unroll
             for (int w = 0; w < 2 * G; ++w)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float k16 = k & 1 ? 1.0f : 16.0f;
+                    const float k16 = k & 1 || !kNormal ? 1.0f : 16.0f;
                     const float p0 = x[w][k] * k16, p1 = x[w][k + 4] * k16;
                     uint32_t v = half2_bits(p0, p1);
                     if constexpr (kPlanes == 2) {
@@ -866,9 +868,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const int w = 2 * q + (step >> 1), shift = 8 * (step & 1);
-                            const uint32_t lo = kw[k][0][w] >> shift, hi = kw[k][1][w] >> shift;
-                            const uint32_t f[4] = {codes<true>(lo, kEven), codes<true>(hi, kEven),
-                                                   codes<true>(lo, kOdd), codes<true>(hi, kOdd)};
+                            uint32_t f[4];      // 16-bit types: even nibbles moved up to where odd ones are
+                            if constexpr (kNormal) {
+                                const uint32_t lo = kw[k][0][w] >> shift, hi = kw[k][1][w] >> shift;
+                                f[0] = codes<true>(lo, kEven), f[1] = codes<true>(hi, kEven);
+                                f[2] = codes<true>(lo, kOdd), f[3] = codes<true>(hi, kOdd);
+                            } else {
+                                const uint32_t lo = kw[k][0][w], hi = kw[k][1][w];
+                                f[0] = (shift ? lo >> 4 : lo << 4) & kOdd, f[1] = (shift ? hi >> 4 : hi << 4) & kOdd;
+                                f[2] = lo >> shift & kOdd, f[3] = hi >> shift & kOdd;
+                            }
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 const uint32_t(&b)[2] = qb[n][2 * w + (step & 1)];
@@ -896,7 +905,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                                 const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&kp[q]));
                                 const float (&t)[4] = acc[k][i / kE][q];
                                 const float d = kPlanes == 2 ? fmaf(t[2 * h + 1], kLo, t[2 * h]) : t[2 * h + i % kE];
-                                const float zero = fmaf(p.x, 8.0f, p.y);
+                                const float zero = kNormal ? fmaf(p.x, 8.0f, p.y) : p.y;
                                 s = q == 0 ? zero * qs[i][q] : fmaf(zero, qs[i][q], s);
                                 s = fmaf(p.x, d, s);
                             }
@@ -975,7 +984,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
 #pragma unroll
                         for (int q = 0; q < G; ++q) {
                             w0[i][q] *= keep;
-                            if constexpr (kPlanes == 1) {
+                            if constexpr (kOnesSum) {
                                 all[i / kE][q][i % kE] *= keep;
                                 all[i / kE][q][2 + i % kE] *= keep;
                             }
@@ -1052,7 +1061,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                     }
 #pragma unroll
                     for (int q = 0; q < G; ++q) {
-                        if constexpr (kPlanes == 1) {
+                        if constexpr (kOnesSum) {
                             constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
                             for (int n = 0; n < NT; ++n) mma_f16(all[n][q], kOnes, pb[k][n][q][0], pb[k][n][q][1]);
@@ -1087,7 +1096,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm 
                 float z = w0[i][q];
 #pragma unroll
                 for (int k = 4; k < 32; k <<= 1) z += __shfl_xor_sync(0xffffffffu, z, k);
-                if constexpr (kPlanes == 1) z = fmaf(all[i / kE][q][i % kE], -kCentre, z);
+                if constexpr (kOnesSum) z = fmaf(all[i / kE][q][i % kE], -kCentre, z);
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
