@@ -582,11 +582,11 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 //
 // Bound by the serial chain of a pair of granules (products, maximum,
 // exponentials, products) on the 12 warps an SM that registers and the rings
-// leave: about 330 instructions a granule of 2304 bytes, 2.2 of 4 issued a cycle
+// leave: about 310 instructions a granule of 2304 bytes, 2.0 of 4 issued a cycle
 // with 2.8 warps a scheduler, most stalls on the instruction before.  8 requests
 // of 16 k to 131 k tokens, 32 query and 8 key/value heads of 128, f16: 118 us (120
 // in a long run), 509 MB at 4.3 TB/s (the copies alone: 85 us); 64 requests of
-// 100 to 8192, bf16: 47.5 us; one of 640, 16 heads, fp32: 12 us.
+// 100 to 8192, bf16: 47 us; one of 640, 16 heads, fp32: 12 us.
 // NT: column tiles of 8; two take 16 query rows (fp32: 8) per unpacking.
 template <class T, int D, int NT, int kPlanes>
 __global__ void __launch_bounds__(kAttendWarps * 32, NT == 1 ? kAttendCtasPerSm : 2) attend_kernel(AttendArgs a) {
